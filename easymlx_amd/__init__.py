@@ -10,7 +10,17 @@ from .caching.paged import AffinePageCacheView, Fp8PageCacheView, PageCacheView,
 from .caching.compiled import CompiledPagedCacheProxy
 from .caching.pagecache import PageCache, PageCacheConfig, validate_cache_dtype
 from .caching.rope import RotaryEmbedding
-from .operations import AttentionOutput, BaseOperation, OperationRegistry, UnifiedAttention, paged_attention
+from .caching.tree import commit_tree
+from .operations import (
+    AttentionOutput,
+    BaseOperation,
+    OperationRegistry,
+    TreeAccept,
+    UnifiedAttention,
+    paged_attention,
+    tree_accept,
+    tree_attention,
+)
 from .quantize import affine_quantize
 
 __all__ = (
@@ -25,9 +35,13 @@ __all__ = (
     "PageCacheView",
     "PageMetadata",
     "RotaryEmbedding",
+    "TreeAccept",
     "UnifiedAttention",
     "affine_quantize",
     "build_query_start_loc",
+    "commit_tree",
     "paged_attention",
+    "tree_accept",
+    "tree_attention",
     "validate_cache_dtype",
 )

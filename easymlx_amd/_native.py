@@ -76,6 +76,25 @@ SIGNATURES: dict[str, tuple] = {
         _I,
         [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _F, _I, _I, _P, _SZ, _P, _P],
     ),
+    "emx_masked_attention_affine": (
+        _I,
+        [_P, _I, _I, _I] + [_P] * 6 + [_I] * 5 + [_P, _I, _I, _P, _P, _F, _I, _I, _P, _I, _P, _SZ, _P, _P],
+    ),
+    "emx_masked_attention_dense": (
+        _I,
+        [_P, _I, _I, _I, _I, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _F, _I, _I, _P, _I, _P, _SZ, _P, _P],
+    ),
+    "emx_masked_attention_fp8": (
+        _I,
+        [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _I, _P, _I, _I, _P, _P, _F, _I, _I, _P, _I, _P, _SZ, _P, _P],
+    ),
+    "emx_masked_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "emx_tree_positions": (_I, [_P, _P, _I, _I, _P, _P]),
+    "emx_tree_accept": (_I, [_P, _P, _I, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "emx_tree_commit_rows": (
+        _I, [_I, _P, _P, ctypes.c_int64, _I, _I, _P, _I, _I, _P, _P, _I, _P, _P, _P, _I, _P]),
+    "emx_tree_commit_affine": (
+        _I, [_I, _P] + [_I] * 6 + [_P, _I, _I, _P, _P, _I, _P, _P, _P, _I, _P]),
 }
 
 _lock = threading.Lock()

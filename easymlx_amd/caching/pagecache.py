@@ -156,6 +156,13 @@ class PageCache:
         for view in self.views:
             view.copy_blocks(mapping)
 
+    def commit_tree(self, path, accepted, query_start_loc, *, slot_ids=None) -> None:
+        """Keep the accepted path of every drafted tree in every layer
+        (:func:`~easymlx_amd.caching.tree.commit_tree`): up to 32 layers of one shape move in one launch."""
+        from .tree import commit_tree
+
+        commit_tree(self.views, path, accepted, query_start_loc, slot_ids=slot_ids)
+
     def zero_pages(self, page_ids) -> None:
         """The runner's ``_zero_pages`` over every layer (``model_runner.py:1058-1094``)."""
         ids = page_ids

@@ -38,6 +38,10 @@ class PageMetadata:
     sliding_window: int | None = None
     is_single_token_decode: bool = False
     slot_ids: tuple[int, ...] | None = None
+    # not in the reference: the first tokens that stay visible beside the sliding window, and the parents of a step
+    # whose tokens are drafted trees (int32 [total_tokens]: index of the parent within the sequence, -1 a root)
+    sink_tokens: int | None = None
+    tree_parents: tp.Any = None
 
     def with_cache_state(self, *, block_tables, kv_lens, block_size: int) -> "PageMetadata":
         return PageMetadata(
@@ -48,6 +52,8 @@ class PageMetadata:
             sliding_window=self.sliding_window,
             is_single_token_decode=self.is_single_token_decode,
             slot_ids=self.slot_ids,
+            sink_tokens=self.sink_tokens,
+            tree_parents=self.tree_parents,
         )
 
     def with_sliding_window(self, sliding_window: int | None) -> "PageMetadata":
@@ -59,6 +65,8 @@ class PageMetadata:
             sliding_window=sliding_window,
             is_single_token_decode=self.is_single_token_decode,
             slot_ids=self.slot_ids,
+            sink_tokens=self.sink_tokens,
+            tree_parents=self.tree_parents,
         )
 
 
@@ -198,9 +206,11 @@ class PageCacheView:
             raise ValueError("block_tables and kv_lens must be int32")
         return dev
 
-    def _slots(self, slot_ids, qlens):
+    def _slots(self, slot_ids, qlens, tree_parents=None):
         """Slot mapping and position of every written token, by ``emx_cache_slots``; advances ``kv_lens``.
 
+        With ``tree_parents`` a token's position is its sequence's length plus its depth in the tree
+        (``emx_tree_positions``); its slot follows the order of the call either way.
         Returns ``(slot_mapping, slots, positions, query_start_loc)`` as int32
         device tensors.  The only host work is one copy of the call's slot ids
         and query offsets (host data in the reference's API) to the device.
@@ -230,7 +240,22 @@ class PageCacheView:
                 slots.data_ptr(), qsl_d.data_ptr(), n, total, bt.data_ptr(), int(bt.shape[0]), int(bt.shape[1]),
                 self.block_size, self.kv_lens.data_ptr(), mapping.data_ptr(), positions.data_ptr(),
                 _stream_ptr(dev)))
+            if tree_parents is not None:
+                _native.check(_native.load().emx_tree_positions(
+                    tree_parents.data_ptr(), qsl_d.data_ptr(), n, total, positions.data_ptr(), _stream_ptr(dev)))
         return mapping, slots, positions, qsl_d
+
+    def _tree_parents(self, cache_metadata, qlens):
+        """The step's tree parents as an int32 tensor of this cache's device, None without them."""
+        parents = getattr(cache_metadata, "tree_parents", None)
+        if parents is None:
+            return None
+        parents = torch.as_tensor(parents)
+        if parents.ndim != 1 or parents.is_floating_point() or parents.is_complex():
+            raise ValueError("tree_parents must be rank-1 integers: [total_tokens]")
+        if int(parents.shape[0]) != sum(max(0, n) for n in qlens):
+            raise ValueError("tree_parents must hold one parent per token written")
+        return parents.to(device=self.block_tables.device, dtype=torch.int32).contiguous()
 
     def _resolve(self, cache_metadata, slot_ids, query_lens, n_tokens):
         if slot_ids is None:
@@ -326,8 +351,11 @@ class PageCacheView:
     ):
         """Append K/V for the scheduled slots (``cache.py:1088-1306``)."""
         slot_ids, qlens, single = self._resolve(cache_metadata, slot_ids, query_lens, int(queries.shape[0]))
-        slot_mapping, slots, positions, qsl = self._slots(slot_ids, qlens)
-        queries, keys = self._apply_rope(rope, queries, keys, positions, qsl, qlens, single)
+        parents = self._tree_parents(cache_metadata, qlens)
+        slot_mapping, slots, positions, qsl = self._slots(slot_ids, qlens, parents)
+        if parents is not None:  # (a tree's positions do not follow each other: every token with an offset of its own)
+            queries, keys = queries[:len(positions)], keys[:len(positions)]
+        queries, keys = self._apply_rope(rope, queries, keys, positions, qsl, qlens, single or parents is not None)
         if slot_mapping.numel():
             self._write(keys.contiguous(), values.contiguous(), slot_mapping)
         return queries, self.key_cache, self.value_cache, self._resolved(cache_metadata, slots, single, slot_ids)
@@ -404,7 +432,7 @@ class PageCacheView:
                                                                                slot_ids)
             if rc != _native.EMX_ERR_UNSUPPORTED:
                 _native.check(rc)
-        slot_mapping, slots, positions, _ = self._slots(slot_ids, qlens)
+        slot_mapping, slots, positions, _ = self._slots(slot_ids, qlens, self._tree_parents(cache_metadata, qlens))
         lib = _native.load()
         n = int(slot_mapping.numel())
         q_in = queries.contiguous()
@@ -483,6 +511,12 @@ class PageCacheView:
         m = block_mapping_on_device(block_mapping, self.key_cache.device)
         if m.shape[0]:
             self._page_call(_native.load().emx_copy_blocks, m, int(m.shape[0]), staging=True)
+
+    def commit_tree(self, path, accepted, query_start_loc, *, slot_ids=None) -> None:
+        """Keep the accepted path of every drafted tree (:func:`~easymlx_amd.caching.tree.commit_tree`)."""
+        from .tree import commit_tree
+
+        commit_tree([self], path, accepted, query_start_loc, slot_ids=slot_ids)
 
     def gather_kv_cache(self, block_table, cu_seq_lens, *, out_dtype: torch.dtype | None = None):
         """Dense ``(k, v)`` ``[total_tokens, Hkv, D]`` of a ragged batch from the pages (``cache.py:974-1027``).

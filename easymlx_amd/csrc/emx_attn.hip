@@ -24,6 +24,7 @@
 #include "slots.hpp"
 #include "probe.hpp"
 #include "pages.hpp"
+#include "entry.hpp"
 #include "mfma_launch.hpp"
 
 constexpr int kNoallocScratchFloats = 2 * emx::kFp8Parts;  // 2 KiB per stream slot
@@ -553,6 +554,18 @@ int launch_gather(const KV& kv, const int32_t* block_table, int num_seqs, int ma
 }
 
 }  // namespace
+
+namespace emx {  // entry.hpp
+
+int entry_fail(int code, const char* message) { return fail(code, "%s", message); }
+int entry_check_launch(const char* what) { return check_launch(what); }
+int entry_check_attention(const void* q, int num_tokens, int hq, int d, int hkv, int nb, int bs, const int32_t* bt,
+                          int S, int max_blocks, const int32_t* kv_lens, const int32_t* qsl, int decode,
+                          const void* out) {
+  return validate_common(q, num_tokens, hq, d, hkv, nb, bs, bt, S, max_blocks, kv_lens, qsl, decode, out);
+}
+
+}  // namespace emx
 
 extern "C" {
 

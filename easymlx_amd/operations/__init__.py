@@ -11,6 +11,7 @@ from ._base_operation import (
     OperationRequirements,
     RequirementsBuilder,
 )
+from .tree_attention import TreeAccept, tree_accept, tree_attention
 from .unified_attention import UnifiedAttention, UnifiedAttnMetadata, paged_attention
 
 __all__ = (
@@ -23,7 +24,10 @@ __all__ = (
     "OperationRegistry",
     "OperationRequirements",
     "RequirementsBuilder",
+    "TreeAccept",
     "UnifiedAttention",
     "UnifiedAttnMetadata",
     "paged_attention",
+    "tree_accept",
+    "tree_attention",
 )

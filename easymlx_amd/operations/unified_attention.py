@@ -49,6 +49,8 @@ class UnifiedAttnMetadata:
     block_size: int
     sliding_window: int | None = None
     is_single_token_decode: bool = False
+    sink_tokens: int | None = None  # not in the reference, as the next
+    tree_parents: tp.Any = None
 
 
 def _validate_inputs(queries, key_cache, value_cache, block_tables, kv_lens, query_start_loc, affine) -> None:
@@ -170,6 +172,74 @@ def _i32(t, device) -> torch.Tensor:
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
+def _masked_attention(queries, key_cache, value_cache, block_tables, kv_lens, query_start_loc, affine, *,
+                      softmax_scale, sliding_window, sink_tokens, tree_parents, single_token_decode, k_scale, v_scale,
+                      k_scales, k_biases, v_scales, v_biases, bits, group_size, workspace, out) -> torch.Tensor:
+    """The call with sinks or a drafted tree: ``emx_masked_attention_*`` on checked, device-resident arguments."""
+    dev = queries.device
+    total, hq, d = (int(x) for x in queries.shape)
+    caches = [t for t in (key_cache, value_cache, k_scale, v_scale, k_scales, k_biases, v_scales, v_biases)
+              if t is not None]
+    if any(t.device != dev for t in caches):
+        raise ValueError(f"the cache must be on the queries' device {dev}")
+    if out.shape != queries.shape or out.dtype != queries.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be a contiguous tensor of the queries' shape, dtype and device")
+    queries = queries.contiguous()
+    S, max_blocks = int(block_tables.shape[0]), int(block_tables.shape[1])
+    fp8 = not affine and key_cache.dtype == torch.uint8 and k_scale is not None and v_scale is not None
+    if affine:
+        if queries.dtype != torch.float16:
+            raise NotImplementedError("affine paged attention takes fp16 queries")
+        if any(not t.is_contiguous() for t in caches):
+            raise ValueError("affine cache tensors must be contiguous")
+        nb, hkv, bs = int(key_cache.shape[0]), int(key_cache.shape[1]), int(key_cache.shape[2])
+    else:
+        if queries.dtype not in _DTYPE_CODE:
+            raise NotImplementedError(f"unsupported dtype {queries.dtype}")
+        if fp8 and value_cache.dtype != torch.uint8:
+            raise ValueError("an FP8 cache needs uint8 key and value caches")
+        if not fp8 and (key_cache.dtype != queries.dtype or value_cache.dtype != queries.dtype):
+            raise NotImplementedError("dense paged attention needs the cache in the queries' dtype")
+        key_cache, value_cache = key_cache.contiguous(), value_cache.contiguous()
+        nb, bs, hkv = int(key_cache.shape[0]), int(key_cache.shape[1]), int(key_cache.shape[2])
+        if fp8:
+            k_scale = k_scale.to(torch.float32).contiguous()
+            v_scale = v_scale.to(torch.float32).contiguous()
+            if k_scale.numel() != nb or v_scale.numel() != nb:
+                raise ValueError("k_scale/v_scale must hold one scale per block: [num_blocks]")
+    lib = _native.load()
+    with torch.cuda.device(dev):
+        stream = _native.stream_ptr(dev)
+        if workspace is None:
+            workspace = _workspace(dev, stream, _masked_bytes(total, S, hq, hkv, d), own=True)
+        ws_ptr = workspace.data_ptr() if workspace is not None else None
+        ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+        geometry = (block_tables.data_ptr(), S, max_blocks, kv_lens.data_ptr(), query_start_loc.data_ptr(),
+                    float(softmax_scale), int(sliding_window), int(sink_tokens),
+                    None if tree_parents is None else tree_parents.data_ptr(), int(bool(single_token_decode)),
+                    ws_ptr, ws_bytes, out.data_ptr(), stream)
+        if affine:
+            rc = lib.emx_masked_attention_affine(
+                queries.data_ptr(), total, hq, d, key_cache.data_ptr(), k_scales.data_ptr(), k_biases.data_ptr(),
+                value_cache.data_ptr(), v_scales.data_ptr(), v_biases.data_ptr(), nb, bs, hkv, int(bits),
+                int(group_size), *geometry)
+        elif fp8:
+            rc = lib.emx_masked_attention_fp8(
+                queries.data_ptr(), total, hq, d, _DTYPE_CODE[queries.dtype], key_cache.data_ptr(),
+                value_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, bs, hkv, *geometry)
+        else:
+            rc = lib.emx_masked_attention_dense(
+                queries.data_ptr(), total, hq, d, _DTYPE_CODE[queries.dtype], key_cache.data_ptr(),
+                value_cache.data_ptr(), nb, bs, hkv, *geometry)
+        _native.check(rc)
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _masked_bytes(total: int, S: int, hq: int, hkv: int, d: int) -> int:
+    return int(_native.load().emx_masked_workspace_bytes(total, S, hq, hkv, d))
+
+
 def paged_attention(
     queries: torch.Tensor,
     key_cache: torch.Tensor,
@@ -180,6 +250,8 @@ def paged_attention(
     *,
     softmax_scale: float | None = None,
     sliding_window: int | None = None,
+    sink_tokens: int | None = None,
+    tree_parents=None,
     single_token_decode: bool | None = None,
     k_scale: torch.Tensor | None = None,
     v_scale: torch.Tensor | None = None,
@@ -204,6 +276,10 @@ def paged_attention(
     ``key_cache [nb, Hkv, bs, D*bits/32]``, ``value_cache [nb, Hkv, bs/T, D, T*bits/32]``
     (``T = min(bs, 256/bits)``),
     scales/biases ``[nb, Hkv, D/group_size, bs]``.
+
+    ``sink_tokens`` (no counterpart in the reference): with a ``sliding_window`` the first ``sink_tokens`` keys of a
+    sequence stay visible beside the window.  ``tree_parents``: the call's tokens are drafted trees
+    (:func:`~easymlx_amd.operations.tree_attention.tree_attention`).
 
     Returns ``[total_tokens, num_q_heads, head_dim]`` in the queries' dtype.
     """
@@ -232,14 +308,32 @@ def paged_attention(
         softmax_scale = 1.0 / math.sqrt(d)
     if sliding_window is None:
         sliding_window = 0
+    sink_tokens = 0 if sink_tokens is None else int(sink_tokens)
+    if sink_tokens < 0:
+        raise ValueError(f"sink_tokens must be >= 0, got {sink_tokens}")
+    if tree_parents is not None:
+        tree_parents = torch.as_tensor(tree_parents)
+        if tree_parents.ndim != 1 or int(tree_parents.shape[0]) != total:
+            raise ValueError("tree_parents must be rank-1: [total_tokens]")
+        if total and (tree_parents.is_floating_point() or tree_parents.is_complex()):
+            raise ValueError("tree_parents must be integers")
+        tree_parents = _i32(tree_parents, dev)
+        single_token_decode = False
     if out is None:
-        out = torch.empty_like(queries)
+        out = torch.empty_like(queries, memory_format=torch.contiguous_format)
     if total == 0:
         return out.zero_()
     if single_token_decode is None:
         single_token_decode = _is_single_token_decode(query_start_loc, total)
     if dev.type != "cuda":
         raise RuntimeError("paged_attention runs on the GPU only; queries are on " + str(dev))
+    if tree_parents is not None or (sink_tokens > 0 and sliding_window > 0):
+        return _masked_attention(
+            queries, key_cache, value_cache, block_tables, kv_lens, query_start_loc, affine,
+            softmax_scale=softmax_scale, sliding_window=sliding_window, sink_tokens=sink_tokens,
+            tree_parents=tree_parents, single_token_decode=single_token_decode, k_scale=k_scale, v_scale=v_scale,
+            k_scales=k_scales, k_biases=k_biases, v_scales=v_scales, v_biases=v_biases, bits=bits,
+            group_size=group_size, workspace=workspace, out=out)
     queries = queries.contiguous()
     lib = _native.load()
     stream = _native.stream_ptr(dev)
@@ -365,6 +459,8 @@ class UnifiedAttention(BaseOperation):
         kwargs: dict[str, tp.Any] = {
             "softmax_scale": scale,
             "sliding_window": cache_metadata.sliding_window,
+            "sink_tokens": getattr(cache_metadata, "sink_tokens", None),
+            "tree_parents": getattr(cache_metadata, "tree_parents", None),
             "single_token_decode": bool(cache_metadata.is_single_token_decode),
         }
         if cache_view is not None and getattr(cache_view, "is_affine", False):

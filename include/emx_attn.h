@@ -479,6 +479,115 @@ int emx_paged_attention_fp8(const void* queries, int num_tokens, int num_q_heads
                             int single_token_decode, void* workspace, size_t workspace_bytes, void* out,
                             void* stream);
 
+/*
+ * Masked paged attention: what the three emx_paged_attention_* calls compute, over the same
+ * caches, for rows that see more or less than a causal run of keys.
+ *
+ * Query i of a sequence (kv_len keys, q query tokens) stands at past + i, past = kv_len - q,
+ * and sees the keys at positions k <= past + i.  With sliding_window > 0 only those with
+ * k > past + i - sliding_window or k < sink_tokens: the first tokens stay visible beside the
+ * window.  (sink_tokens without a window changes nothing.)
+ *
+ * tree_parents int32 [num_tokens] (device; null: none) makes the q tokens of every sequence a
+ * drafted tree: entry t is the index, within its own sequence, of row t's parent, an earlier
+ * row; any other value makes a root.  Node i then stands at past + depth(i); it sees the keys
+ * before `past`, and of the tree's own keys its own and those of its ancestors, whose places are
+ * past + their depths (window and sinks go by places).  A tree may have any number of nodes.
+ *
+ * A row that sees no key gives zeros, as do rows that no sequence holds.  Keys that a row does
+ * not see do not change its result, whatever they hold.  softmax_scale must be positive.
+ *
+ * workspace: emx_masked_workspace_bytes(...) bytes (the first
+ * emx_paged_workspace_zeroed_bytes() of them are not used, so that one buffer serves these
+ * and the paged calls of a stream); no zero fill is needed.  With less, or null, tiles of
+ * many keys are not cut over workgroups: slower for few rows over long contexts, the same
+ * results but for rounding.  Calls sharing a workspace must not overlap.  Results do not depend
+ * on the order in which workgroups run.
+ * fp16 / bf16 (queries' type) over unquantized caches, fp16 over FP8 and affine pages with
+ * head_dim 64, 128 or 256, pages of a multiple of 8 tokens and 16-byte aligned tensors run on
+ * the matrix units; other shapes, and fp32, on one wave per (token, kv head).
+ * No counterpart in the reference.
+ */
+int emx_masked_attention_affine(const void* queries, int num_tokens, int num_q_heads, int head_dim,
+                                const uint32_t* k_codes, const void* k_scales, const void* k_biases,
+                                const uint32_t* v_codes, const void* v_scales, const void* v_biases, int num_blocks,
+                                int page_size, int num_kv_heads, int bits, int group_size,
+                                const int32_t* block_tables, int num_seqs, int max_blocks_per_seq,
+                                const int32_t* kv_lens, const int32_t* query_start_loc, float softmax_scale,
+                                int sliding_window, int sink_tokens, const int32_t* tree_parents,
+                                int single_token_decode, void* workspace, size_t workspace_bytes, void* out,
+                                void* stream);
+int emx_masked_attention_dense(const void* queries, int num_tokens, int num_q_heads, int head_dim, int dtype,
+                               const void* key_cache, const void* value_cache, int num_blocks, int page_size,
+                               int num_kv_heads, const int32_t* block_tables, int num_seqs, int max_blocks_per_seq,
+                               const int32_t* kv_lens, const int32_t* query_start_loc, float softmax_scale,
+                               int sliding_window, int sink_tokens, const int32_t* tree_parents,
+                               int single_token_decode, void* workspace, size_t workspace_bytes, void* out,
+                               void* stream);
+int emx_masked_attention_fp8(const void* queries, int num_tokens, int num_q_heads, int head_dim, int dtype,
+                             const uint8_t* key_cache, const uint8_t* value_cache, const float* k_scale,
+                             const float* v_scale, int num_blocks, int page_size, int num_kv_heads,
+                             const int32_t* block_tables, int num_seqs, int max_blocks_per_seq,
+                             const int32_t* kv_lens, const int32_t* query_start_loc, float softmax_scale,
+                             int sliding_window, int sink_tokens, const int32_t* tree_parents,
+                             int single_token_decode, void* workspace, size_t workspace_bytes, void* out,
+                             void* stream);
+
+/*
+ * Bytes of workspace with which emx_masked_attention_* cuts tiles of many keys (0: the call has
+ * tiles enough, or a shape outside the matrix units).
+ */
+size_t emx_masked_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
+
+/*
+ * Positions of a drafted tree's tokens: positions[t], as emx_cache_slots gives it (first + index
+ * in the call's sequence), becomes first + depth(t), the place at which the token stands if
+ * its path is accepted and by which its key and query are rotated.  tree_parents as above,
+ * query_start_loc int32 [num_slots + 1] on the device.
+ */
+int emx_tree_positions(const int32_t* tree_parents, const int32_t* query_start_loc, int num_slots, int num_tokens,
+                       int32_t* positions, void* stream);
+
+/*
+ * The accepted path of every drafted tree.  tokens [num_tokens]: the trees' tokens; targets
+ * [num_tokens]: the token that the model chooses after each node (both of token_bytes 4 or 8, device).
+ * Node 0, the token that the last step chose, is taken; then of the last taken node's children
+ * the first (lowest row) whose token is the target after that node, until none is.
+ * path int32 [num_tokens]: row query_start_loc[s] + k holds the index in the tree of the
+ * path's node k, the rows behind a path and those of no tree -1.  accepted int32 [num_slots]: nodes of each
+ * path (0 for an empty tree).  next_tokens [num_slots], of token_bytes: the target after the
+ * path's last node (-1 for an empty tree).
+ */
+int emx_tree_accept(const void* tokens, const void* targets, int token_bytes, const int32_t* tree_parents,
+                    const int32_t* query_start_loc, int num_slots, int num_tokens, int32_t* path, int32_t* accepted,
+                    void* next_tokens, void* stream);
+
+/*
+ * Keeps the accepted paths in the cache of num_layers layers of one shape.  Tree i is the last
+ * q = query_start_loc[i + 1] - query_start_loc[i] tokens of sequence slot_ids[i] (null: i), at positions
+ * first = kv_lens[s] - q ...  The rows of node path[query_start_loc[i] + k], k < accepted[i],
+ * move to position first + k, and kv_lens[s] becomes first + accepted[i].  A path ascends
+ * (path[k] >= k; an entry that does not, or lies outside the tree, is left where it is), a
+ * sequence appears once, and its tree's pages are its own.  Rows on pages outside the pool are skipped.
+ * key_caches, value_caches, block_tables, kv_lens: host arrays of num_layers device pointers
+ * (layers may share tables and lengths; shared lengths change once).  row_bytes: of a token's
+ * [Hkv, head_dim] row in the token-major caches [num_blocks, page_size, Hkv, head_dim].  FP8
+ * codes move as they are: a tree's rows are written by one call with one scale, and a page that
+ * holds any of them has a scale of at least that.
+ * _affine: arrays holds six pointers per layer (key codes, value codes, k_scales, k_biases,
+ * v_scales, v_biases).
+ */
+int emx_tree_commit_rows(int num_layers, void* const* key_caches, void* const* value_caches, int64_t row_bytes,
+                         int page_size, int num_blocks, const int32_t* const* block_tables, int num_seqs,
+                         int max_blocks_per_seq, int32_t* const* kv_lens, const int32_t* slot_ids, int num_slots,
+                         const int32_t* path, const int32_t* accepted, const int32_t* query_start_loc, int num_tokens,
+                         void* stream);
+int emx_tree_commit_affine(int num_layers, void* const* arrays, int num_kv_heads, int head_dim, int bits,
+                           int group_size, int page_size, int num_blocks, const int32_t* const* block_tables,
+                           int num_seqs, int max_blocks_per_seq, int32_t* const* kv_lens, const int32_t* slot_ids,
+                           int num_slots, const int32_t* path, const int32_t* accepted,
+                           const int32_t* query_start_loc, int num_tokens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
