@@ -9,7 +9,7 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 SOURCES = [os.path.join(CSRC, f) for f in ("emx_attn.hip", "emx_mfma.hip", "emx_masked.hip", "emx_masked_affine.hip",
-                                        "emx_tree.hip")]
+                                        "emx_masked_rows.hip", "emx_tree.hip")]
 DEPENDS = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".hpp", ".hip"))]
 OUT = os.path.join(_HERE, "_lib", "libemx_attn.so")
 

@@ -47,6 +47,7 @@ struct DecodeMfmaArgs {
   int hc, nhc;       // query heads per unit (<= 16) and units per kv head
   uint32_t inv_bs;   // ceil(2^32 / bs)
   int T;             // query rows
+  int sinks;         // SINKS: the tokens that stay visible before a window (> 0; a.window > 0)
 };
 
 // A unit that is cut costs its merge (a round trip through memory, the atomic and the
@@ -152,8 +153,15 @@ __device__ __forceinline__ bool write4(const f32x4 O, const float L, QT* out) {
 // sequences before s, kvl[s] = clamped kv_len (-1: not a single-token row of the call's T), qrw[s] = query row.
 // (seq_table of decode_affine.hpp with a constant item size: its two divisions by a run-time
 // one and the serial 64-bit range arithmetic were a third of a short call.)
+// SINKS: a unit's items are those that hold sinks before its window's first, then the window's.
 template <int NT>
-__device__ __forceinline__ void decode_mfma_table(const DecodeArgs& a, const int T, int* cum, int* kvl, int* qrw, int* wsum) {
+__device__ __forceinline__ int sink_items(const int sinks, const int kl, const int st) {
+  return min((min(sinks, kl) + NT - 1) / NT, st / NT);
+}
+
+template <int NT, bool SINKS>
+__device__ __forceinline__ void decode_mfma_table(const DecodeArgs& a, const int T, const int sinks, int* cum, int* kvl,
+                                                  int* qrw, int* wsum) {
   const int ch = (a.S + 255) / 256, s0 = threadIdx.x * ch;
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
   int tsum = 0;
@@ -164,7 +172,8 @@ __device__ __forceinline__ void decode_mfma_table(const DecodeArgs& a, const int
     const int q0 = a.qsl ? a.qsl[s] : s, q1 = a.qsl ? a.qsl[s + 1] : s + 1;
     const bool dec = q1 - q0 == 1 && (unsigned)q0 < (unsigned)T;
     const int st = a.window > 0 ? max(0, kl - a.window) : 0;
-    const int n = dec && kl > 0 ? (kl - 1) / NT - st / NT + 1 : 0;
+    int n = dec && kl > 0 ? (kl - 1) / NT - st / NT + 1 : 0;
+    if constexpr (SINKS) n += n > 0 ? sink_items<NT>(sinks, kl, st) : 0;
     kvl[s] = dec ? kl : -1;
     qrw[s] = q0;
     cum[s] = n;  // the count for now
@@ -192,7 +201,10 @@ __device__ __forceinline__ void decode_mfma_table(const DecodeArgs& a, const int
   __syncthreads();
 }
 
-template <class C, int D>
+// SINKS: the first A.sinks tokens are seen beside the window (masked_launch.hpp).  As a tile of masked_mfma, where the
+// rows of a group's heads are one wave's and the other three wait, / here: batch 32 over 4-bit pages, window 4096, four
+// sinks, contexts of 2048 to 16384 (149 MB) 142 / 52 us; batch 48 over bf16 pages of 16, 64 sinks (808 MB) 186 / 166.
+template <class C, int D, bool SINKS = false>
 __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const int bid, const int nblocks) {
   using P = DecodeMfmaCfg<C, D>;
   typedef typename C::Op Op;
@@ -218,7 +230,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
   float* xml = &lds_at<float>(oXml);    // [wave][head][2]
   int& flag = lds_at<int>(oFlag);
   h16* stage = &lds_at<h16>(oStage) + wv * P::STAGE;  // affine: this wave's [array][group][token] scales
-  decode_mfma_table<NT>(a, A.T, cum, kvl, qrw, reinterpret_cast<int*>(xml));
+  decode_mfma_table<NT, SINKS>(a, A.T, SINKS ? A.sinks : 0, cum, kvl, qrw, reinterpret_cast<int*>(xml));
   const int S = a.S, HG = a.Hq / a.Hkv, Hu = a.Hkv * A.nhc;
   {  // decoded sequences without a live token produce zeros (the reference's l == 0 case)
     const int per_seq = a.Hq * D / 8;
@@ -240,7 +252,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
     const int si = c + lane;
     const int n = si < S ? cum[si + 1] - cum[si] : 0;
     nmax = max(nmax, n);
-    if (n > 0) solo = solo && (kvl[si] - 1) / P::NTW == start_of(kvl[si]) / P::NTW;
+    if (n > 0)
+      solo = solo && (SINKS ? kvl[si] <= P::NTW : (kvl[si] - 1) / P::NTW == start_of(kvl[si]) / P::NTW);
   }
   nmax = uru((int)wave_max((float)nmax));
   solo = __all(solo);
@@ -313,7 +326,14 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
     int s, y, j, n, kl, st, tb;
     int has;  // inside the range
   };
-  auto tb_of = [&](int st, int jx) { return solo ? st / P::NTW * P::NTW : (st / NT + jx) * NT + P::NTW * wv; };
+  auto tb_of = [&](int kl, int st, int jx) {
+    if constexpr (SINKS) {
+      const int ns = sink_items<NT>(A.sinks, kl, st);
+      return solo ? 0 : (jx < ns ? jx : st / NT + jx - ns) * NT + P::NTW * wv;
+    } else {
+      return solo ? st / P::NTW * P::NTW : (st / NT + jx) * NT + P::NTW * wv;
+    }
+  };
   Item it0;
   {
     it0.s = seq_of(g0);
@@ -323,7 +343,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
     it0.j = r - it0.y * it0.n;
     it0.kl = uru(kvl[it0.s]);
     it0.st = start_of(it0.kl);
-    it0.tb = tb_of(it0.st, it0.j);
+    it0.tb = tb_of(it0.kl, it0.st, it0.j);
     it0.has = true;
   }
   // the item after x, g being x's index; past the range x again with has = false
@@ -343,7 +363,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
         r.st = start_of(r.kl);
       }
     }
-    r.tb = tb_of(r.st, r.j);
+    r.tb = tb_of(r.kl, r.st, r.j);
     return r;
   };
 
@@ -572,7 +592,9 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
     bool okp = ok_blk(lc.blk[1]);
 #pragma unroll
     for (int n = 2; n < P::NL; ++n) okp = okp && ok_blk(lc.blk[n]);
-    const bool full = tb >= start_k && tb + P::NTW <= kv_len && __all(okp);
+    // (SINKS: a token before the window is seen if it is a sink)
+    auto seen = [&](const int p) { return (p >= start_k || (SINKS && p < A.sinks)) && p < kv_len; };
+    const bool full = (tb >= start_k || (SINKS && tb + P::NTW <= A.sinks)) && tb + P::NTW <= kv_len && __all(okp);
     if constexpr (C::kAffine) {
       // ---- this item's scales to the wave's LDS slot; those of tokens outside
       // [start_k, kv_len) or on an invalid page (which may hold anything) as zeros
@@ -584,8 +606,8 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
         if (!full) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const bool ok0 = p0 + 2 * e >= start_k && p0 + 2 * e < kv_len && ok_blk(lc.blk[2 + i]);
-            const bool ok1 = p0 + 2 * e + 1 >= start_k && p0 + 2 * e + 1 < kv_len && ok_blk(lc.blk[2 + i]);
+            const bool ok0 = seen(p0 + 2 * e) && ok_blk(lc.blk[2 + i]);
+            const bool ok1 = seen(p0 + 2 * e + 1) && ok_blk(lc.blk[2 + i]);
             x[e] &= (ok0 ? 0x0000FFFFu : 0u) | (ok1 ? 0xFFFF0000u : 0u);
           }
         }
@@ -659,7 +681,7 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
 #pragma unroll
       for (int e = 0; e < NV; ++e) {
         const int p = tb + (C::kAffine ? NV * jj + e : 16 * (e >> 2) + 4 * jj + (e & 3));
-        if (p < start_k || p >= kv_len || !ok_blk(lc.blk[C::kAffine ? 1 : 2 + (e >> 2)])) sc[e] = -INFINITY;
+        if (!seen(p) || !ok_blk(lc.blk[C::kAffine ? 1 : 2 + (e >> 2)])) sc[e] = -INFINITY;
       }
     }
     float tmax = -INFINITY;
@@ -840,11 +862,20 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
         if (!solo) __syncthreads();
         const int b0 = start_k / NT - unit_first;  // item g of the unit: tokens from (b0 + g) NT
         // (a piece's sums are of p = 2^(x - m + kPBias), as the others')
-        const int k0 = max(start_k, (b0 + seg0) * NT), k1 = min(kv_len, (b0 + g + 1) * NT);
+        int k0 = max(start_k, (b0 + seg0) * NT), k1 = min(kv_len, (b0 + g + 1) * NT);
+        if constexpr (SINKS) {  // the pieces' first and last items; the gap between sinks and window lies inside or outside
+          const int ns = sink_items<NT>(A.sinks, kv_len, start_k);
+          const int ja = seg0 - unit_first, jb = g - unit_first;
+          k0 = (ja < ns ? ja : start_k / NT + ja - ns) * NT;
+          k1 = min(kv_len, ((jb < ns ? jb : start_k / NT + jb - ns) + 1) * NT);
+        }
         for (int h = solo ? 0 : wv; h < nh; h += solo ? 1 : 4) {
           float mr, lr, x[D / 64];
           const QT* qp = reinterpret_cast<const QT*>(a.q) + ((size_t)qrw[s] * a.Hq + (size_t)kvh * HG + h0 + h) * D;
-          attend_row<C, D>(a, s, kvh, qp, k0, k1, mr, lr, x, lane);
+          if constexpr (SINKS)
+            attend_row<C, D, true>(a, s, kvh, qp, k0, k1, mr, lr, x, lane, A.sinks, max(start_k, A.sinks));
+          else
+            attend_row<C, D>(a, s, kvh, qp, k0, k1, mr, lr, x, lane);
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) {
             if (whole)
@@ -959,9 +990,9 @@ __device__ __forceinline__ void decode_mfma_body(const DecodeMfmaArgs& A, const 
 }
 
 // (D = 256 holds 64 words of V and 64 of K per lane: one workgroup per compute unit, no spills)
-template <class C, int D>
+template <class C, int D, bool SINKS = false>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void decode_mfma(DecodeMfmaArgs a) {
-  decode_mfma_body<C, D>(a, blockIdx.x, gridDim.x);
+  decode_mfma_body<C, D, SINKS>(a, blockIdx.x, gridDim.x);
 }
 
 }  // namespace emx

@@ -33,6 +33,9 @@ MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, bool cut) {
 
 namespace {
 
+// Where a call's partials start in its workspace: behind the counters, which are zero between calls.
+size_t workspace_base() { return (emx_paged_workspace_zeroed_bytes() + 255) & ~(size_t)255; }
+
 bool head_ok(int D) { return D == 64 || D == 128 || D == 256; }
 
 // The call's geometry, and the rule, as the entry points receive them.
@@ -94,7 +97,16 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
   m.window = c.mask.window;
   if (g.S <= 0 || !mfma_ok(m) || (long long)g.nb * g.bs * (m.kind == KvKind::affine ? g.Hkv : 1) >= (1LL << 31))
     return false;
-  const size_t base = (emx_paged_workspace_zeroed_bytes() + 255) & ~(size_t)255;
+  const size_t base = workspace_base();
+  // rows of one token: the split-K decode (a tile of the kernel below would hold a group's heads alone)
+  const size_t rows = g.decode && c.mask.sinks > 0 && !c.mask.parents
+                          ? decode_mfma_partial_bytes(g.S, g.Hq, g.Hkv, g.D) : 0;
+  if (rows && c.ws && c.ws_bytes >= base + rows) {
+    launch_masked_rows(m, c.mask.sinks, static_cast<int*>(c.ws),
+                       reinterpret_cast<float*>(static_cast<char*>(c.ws) + base), c.st);
+    *rc = entry_check_launch("decode_mfma (sinks)");
+    return true;
+  }
   MaskedShape shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, true);
   if (shape.tokb == 0) return false;
   if (shape.part_bytes && (!c.ws || c.ws_bytes < base + shape.part_bytes))
@@ -151,8 +163,10 @@ size_t emx_masked_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads,
   if (num_tokens <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       !head_ok(head_dim))
     return 0;
-  const size_t part = masked_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, true).part_bytes;
-  return part ? ((emx_paged_workspace_zeroed_bytes() + 255) & ~(size_t)255) + part : 0;
+  size_t part = masked_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, true).part_bytes;
+  if (num_tokens == num_seqs)
+    part = std::max(part, decode_mfma_partial_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim));
+  return part ? workspace_base() + part : 0;
 }
 
 int emx_masked_attention_affine(const void* queries, int num_tokens, int num_q_heads, int head_dim,

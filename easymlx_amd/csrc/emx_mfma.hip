@@ -12,7 +12,6 @@ namespace emx {
 namespace {
 
 constexpr int kDecodeMfmaWGs = 512;  // persistent grid: two workgroups per compute unit ..
-int decode_wgs(int D) { return D == 256 ? kDecodeMfmaWGs / 2 : kDecodeMfmaWGs; }  // .. or the one that fits
 
 bool head_ok(int D) { return D == 64 || D == 128 || D == 256; }
 int head_chunk(int Hq, int Hkv) { return std::min(Hq / Hkv, 16); }
@@ -42,6 +41,8 @@ DecodeMfmaFn decode_fn(const MfmaCall& c) {
 
 }  // namespace
 
+int decode_mfma_wgs(int D) { return D == 256 ? kDecodeMfmaWGs / 2 : kDecodeMfmaWGs; }  // .. or the one that fits
+
 bool mfma_ok(const MfmaCall& c) {
   // page_of() is exact for power-of-two pages, and for the others while position * bs < 2^32
   const bool pages = c.bs % 8 == 0 && ((c.bs & (c.bs - 1)) == 0 || (long long)c.max_blocks * c.bs * c.bs < (1LL << 32));
@@ -63,7 +64,7 @@ size_t decode_mfma_partial_bytes(int S, int Hq, int Hkv, int D) {
   return slots * head_chunk(Hq, Hkv) * (D + 2) * sizeof(float);
 }
 
-static DecodeMfmaArgs decode_args(const MfmaCall& c, int* ws_cnt, float* partials) {
+DecodeMfmaArgs decode_mfma_args(const MfmaCall& c, int* ws_cnt, float* partials) {
   DecodeMfmaArgs A{};
   DecodeArgs& a = A.d;
   a.q = static_cast<const h16*>(c.q);
@@ -99,7 +100,7 @@ static DecodeMfmaArgs decode_args(const MfmaCall& c, int* ws_cnt, float* partial
 }
 
 void launch_decode_mfma(const MfmaCall& c, int* ws_cnt, float* partials, hipStream_t st) {
-  hipLaunchKernelGGL(decode_fn(c), dim3(decode_wgs(c.D)), dim3(256), 0, st, decode_args(c, ws_cnt, partials));
+  hipLaunchKernelGGL(decode_fn(c), dim3(decode_mfma_wgs(c.D)), dim3(256), 0, st, decode_mfma_args(c, ws_cnt, partials));
 }
 
 namespace {
@@ -155,7 +156,7 @@ size_t mixed_mfma_part_bytes(int T, int S, int Hq, int Hkv, int D) {
 
 void launch_mixed_mfma(const MfmaCall& c, int* ws_cnt, float* partials, int* ws_part_cnt, float* part,
                        hipStream_t st) {
-  const DecodeMfmaArgs d = decode_args(c, ws_cnt, partials);
+  const DecodeMfmaArgs d = decode_mfma_args(c, ws_cnt, partials);
   PrefillMfmaArgs p{};
   p.d = d.d;
   p.inv_bs = d.inv_bs;

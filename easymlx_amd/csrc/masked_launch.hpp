@@ -67,6 +67,9 @@ struct MaskedShape {
 };
 MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, bool cut);
 
+// Single-token rows (c.qsl null) with a window and sinks > 0; buffers as launch_decode_mfma's (emx_masked_rows.hip).
+void launch_masked_rows(const MfmaCall& c, int sinks, int* ws_cnt, float* partials, hipStream_t st);
+
 void launch_masked_affine(const MfmaCall& c, const MaskedArgs& a, int ct, hipStream_t st);  // emx_masked_affine.hip
 
 }  // namespace emx

@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256, 2) void masked_mfma(MaskedArgs A) {
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, jj = lane >> 4;
 
-  // LDS, carved from the shared arena
+  // LDS: one array of the size needed (not the shared arena: three workgroups fit a compute unit)
   constexpr bool AFF = C::kAffine;
   constexpr int G = [] {
     if constexpr (C::kAffine) return P::G;
@@ -347,15 +347,15 @@ __global__ __launch_bounds__(256, 2) void masked_mfma(MaskedArgs A) {
   constexpr int oVe = lds_next(oKe, 2 * NT * P::KSTR), oKsf = lds_next(oVe, 2 * (AFF ? D : NT) * P::VSTR);
   constexpr int oVsf = lds_next(oKsf, 4 * G * NT), oVbf = lds_next(oVsf, 4 * G * NT);
   constexpr int oKbe = lds_next(oVbf, AFF ? 4 * G * NT : 0), oEnd = lds_next(oKbe, AFF ? 16 * NT : 0);
-  static_assert(oEnd <= kArenaBytes, "LDS arena too small");
-  int* lpar = &lds_at<int>(oPar);
-  int* wred = &lds_at<int>(oWred);
-  uint16_t* ke = &lds_at<uint16_t>(oKe);  // [key][KSTR]
-  uint16_t* ve = &lds_at<uint16_t>(oVe);  // [key][VSTR]; affine: [dim][VSTR]
-  float* ksf = &lds_at<float>(oKsf);      // key scale of each key; affine: [group][NT], * 2^kCodeExp
-  float* vsf = &lds_at<float>(oVsf);      // value scales / 2^vexp
-  float* vbf = &lds_at<float>(oVbf);      // affine: value biases
-  h16* kbe = &lds_at<h16>(oKbe);          // affine: bias operand rows, key bias of group g at 2 g, 2 g + 1
+  __shared__ __attribute__((aligned(16))) unsigned char lds[oEnd];
+  int* lpar = reinterpret_cast<int*>(lds + oPar);
+  int* wred = reinterpret_cast<int*>(lds + oWred);
+  uint16_t* ke = reinterpret_cast<uint16_t*>(lds + oKe);  // [key][KSTR]
+  uint16_t* ve = reinterpret_cast<uint16_t*>(lds + oVe);  // [key][VSTR]; affine: [dim][VSTR]
+  float* ksf = reinterpret_cast<float*>(lds + oKsf);      // key scale of each key; affine: [group][NT], * 2^kCodeExp
+  float* vsf = reinterpret_cast<float*>(lds + oVsf);      // value scales / 2^vexp
+  float* vbf = reinterpret_cast<float*>(lds + oVbf);      // affine: value biases
+  h16* kbe = reinterpret_cast<h16*>(lds + oKbe);          // affine: bias operand rows, key bias of group g at 2 g, 2 g + 1
 
   const int kvh = blockIdx.x % a.Hkv, bid = blockIdx.x / a.Hkv;
   const MaskedUnit u = masked_plan<NT>(A, bid, false, wred);

@@ -130,9 +130,11 @@ __device__ __forceinline__ int page_of(const int p, const uint32_t inv) { return
 // probabilities.  With an infinite value in one page: a context of 1024 tokens, fp16, D 64, 26 us (a
 // key at a time, over the merged row: 812), batch 32 of 512 .. 4096 tokens, bf16, 289 (2000), four
 // 512-token chunks beside 28 rows 7500 (34700; 18500 on paged_generic, finite or not).
-template <class C, int D>
+// GAP: the keys [gap0, gap1) are left out (between a window and the sinks before it).
+template <class C, int D, bool GAP = false>
 __device__ void attend_row(const DecodeArgs& a, const int s, const int kvh, const typename C::QT* q, const int k0,
-                           const int k1, float& m, float& l, float (&acc)[D / 64], const int lane) {
+                           const int k1, float& m, float& l, float (&acc)[D / 64], const int lane, const int gap0 = 0,
+                           const int gap1 = 0) {
   constexpr int N = D / 64;
   const auto kv = kv_loader<C>(a, D);
   float qv[N];
@@ -145,8 +147,9 @@ __device__ void attend_row(const DecodeArgs& a, const int s, const int kvh, cons
   }
 #pragma unroll 1
   for (int base = k0 & ~63; base < k1; base += 64) {
+    if (GAP && base >= gap0 && base + 64 <= gap1) continue;
     const int k = base + lane;
-    const int blk = k >= k0 && k < k1 ? a.block_tables[(size_t)s * a.max_blocks + k / a.bs] : -1;
+    const int blk = k >= k0 && k < k1 && (!GAP || k < gap0 || k >= gap1) ? a.block_tables[(size_t)s * a.max_blocks + k / a.bs] : -1;
     const bool ok = (unsigned)blk < (unsigned)a.nb;
     const uint64_t okm = __ballot(ok);
     float x = 0.f;

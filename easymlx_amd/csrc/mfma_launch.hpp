@@ -37,6 +37,9 @@ bool mfma_ok(const MfmaCall& c);
 // Bytes the decode's partials take after the workspace's fixed region (0: shape not taken).
 size_t decode_mfma_partial_bytes(int S, int Hq, int Hkv, int D);
 // ws_cnt: the workspace's unit counters; partials: decode_mfma_partial_bytes bytes.
+struct DecodeMfmaArgs;  // decode_mfma.hpp
+DecodeMfmaArgs decode_mfma_args(const MfmaCall& c, int* ws_cnt, float* partials);
+int decode_mfma_wgs(int D);  // workgroups of its grid
 void launch_decode_mfma(const MfmaCall& c, int* ws_cnt, float* partials, hipStream_t st);
 
 // A ragged call (qsl given): rows of longer queries, and single-token rows beside them.

@@ -497,11 +497,11 @@ int emx_paged_attention_fp8(const void* queries, int num_tokens, int num_q_heads
  * A row that sees no key gives zeros, as do rows that no sequence holds.  Keys that a row does
  * not see do not change its result, whatever they hold.  softmax_scale must be positive.
  *
- * workspace: emx_masked_workspace_bytes(...) bytes (the first
- * emx_paged_workspace_zeroed_bytes() of them are not used, so that one buffer serves these
- * and the paged calls of a stream); no zero fill is needed.  With less, or null, tiles of
- * many keys are not cut over workgroups: slower for few rows over long contexts, the same
- * results but for rounding.  Calls sharing a workspace must not overlap.  Results do not depend
+ * workspace: emx_masked_workspace_bytes(...) bytes, the first
+ * emx_paged_workspace_zeroed_bytes() of them zero before its first use, as for
+ * emx_paged_attention_affine: one buffer serves these and the paged calls of a stream.  With less,
+ * or null, the work of a row is not spread over workgroups: slower for few rows over long
+ * contexts, the same results but for rounding.  Calls sharing a workspace must not overlap.  Results do not depend
  * on the order in which workgroups run.
  * fp16 / bf16 (queries' type) over unquantized caches, fp16 over FP8 and affine pages with
  * head_dim 64, 128 or 256, pages of a multiple of 8 tokens and 16-byte aligned tensors run on
@@ -534,8 +534,8 @@ int emx_masked_attention_fp8(const void* queries, int num_tokens, int num_q_head
                              void* stream);
 
 /*
- * Bytes of workspace with which emx_masked_attention_* cuts tiles of many keys (0: the call has
- * tiles enough, or a shape outside the matrix units).
+ * Bytes of workspace with which emx_masked_attention_* spreads long rows over workgroups (0: the
+ * call has tiles enough, or a shape outside the matrix units).
  */
 size_t emx_masked_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim);
 

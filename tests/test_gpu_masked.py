@@ -191,6 +191,27 @@ def test_unseen_keys_may_hold_anything(cuda, kind, shape):
     check(b, run(b, cuda, 20, 4), exp)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_decode_rows_beside_anything(cuda, kind):
+    """Rows of one token: junk between sinks and window, and an infinite value among the sinks or in the window."""
+    lens = [700, 40, 1500, 3000]
+    b = batch(kind, [1] * 4, lens, 8, 2, 128, 16, seed=10)
+    exp = expected(b, 600, 70)
+    for s, n in enumerate(lens):
+        for pos in range(70, n - 600):
+            blk, off = where(b, s, pos)
+            b["cache"][0][blk, off], b["cache"][1][blk, off] = float("nan"), float("inf")
+    check(b, run(b, cuda, 600, 70, decode=True), exp)
+    for s, pos in ((2, 69), (3, 2400)):
+        blk, off = where(b, s, pos)
+        b["cache"][1][blk, off, 1, 5] = -float("inf")
+    got = run(b, cuda, 600, 70, decode=True)
+    assert (got[2:, 4:, 5] == -np.inf).all()
+    keep = np.ones_like(exp, bool)
+    keep[2:, 4:, 5] = False
+    check(b, np.where(keep, got, 0), np.where(keep, exp, 0))
+
+
 def test_infinite_value_in_a_cut_tile(cuda):
     """A seen value of infinity among many parts: that dim alone, for the rows that see it."""
     b = batch("f16", [3], [20_000], 4, 1, 128, 16, seed=12)
