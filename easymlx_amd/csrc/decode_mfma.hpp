@@ -201,7 +201,7 @@ __device__ __forceinline__ void decode_mfma_table(const DecodeArgs& a, const int
   __syncthreads();
 }
 
-// SINKS: the first A.sinks tokens are seen beside the window (masked_launch.hpp).  As a tile of masked_mfma, where the
+// SINKS: the first A.sinks tokens are seen beside the window (masked_launch.hpp).  As a tile of masked_wide, where the
 // rows of a group's heads are one wave's and the other three wait, / here: batch 32 over 4-bit pages, window 4096, four
 // sinks, contexts of 2048 to 16384 (149 MB) 142 / 52 us; batch 48 over bf16 pages of 16, 64 sinks (808 MB) 186 / 166.
 template <class C, int D, bool SINKS = false>

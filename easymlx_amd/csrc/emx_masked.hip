@@ -11,23 +11,25 @@
 
 namespace emx {
 
-// Two workgroups of a compute unit; a call of fewer tiles is cut.
-constexpr long kMaskedWGs = 512;
+// Workgroups that the chip holds at once, two to a compute unit; a call of fewer tiles is cut.
+constexpr int kMaskedWGs = 512;
 
 MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, bool cut) {
   MaskedShape m{};
   const int hg = Hq / Hkv;
-  // Query columns per wave: 16 ct.  More columns read each K and V operand from LDS fewer times; at
-  // D 256 the accumulator of 32 columns leaves one wave per SIMD.  Sequences of up to 64 columns
-  // (small trees, decode rows) would leave half of them empty.
-  m.ct = D <= 128 && (hg > 64 || (long)T * hg > 64L * S) ? 2 : 1;
-  if (hg <= 0 || hg > 64 * m.ct || T <= 0 || S <= 0) return MaskedShape{};
-  m.tokb = 64 * m.ct / hg;
+  if (hg <= 0 || T <= 0 || S <= 0) return m;
+  // sequences of up to 64 columns on average (small trees): two waves to a column, half of the keys each
+  m.kw = D <= 128 && hg <= 64 && (long)T * hg <= 64L * S ? 2 : 1;
+  if (hg > 128 / m.kw) return m;
+  m.tokb = 128 / m.kw / hg;
   // a sequence of q query tokens has at most q / tokb + 1 tiles
-  m.tiles = ((long)T + m.tokb - 1) / m.tokb + std::min(S, T);
-  m.share_of = cut && ((long)T + m.tokb - 1) / m.tokb * Hkv < 2 * kMaskedWGs ? (kMaskedWGs + Hkv - 1) / Hkv : 0;
-  m.units = m.tiles + (m.share_of ? 2 * m.share_of + 1 : 0);
-  m.part_bytes = m.share_of ? (size_t)m.units * Hkv * (4 * (m.ct * (D / 16) + 1) * 1024) : 0;
+  const long least = ((long)T + m.tokb - 1) / m.tokb;
+  m.tiles = least + std::min(S, T);
+  if (cut && least * Hkv < 2 * kMaskedWGs) {
+    m.wgs = D == 256 ? kMaskedWGs / 2 : kMaskedWGs;  // (its registers: one workgroup to a compute unit)
+    m.desc_bytes = 16 * (size_t)(1 + m.tiles * Hkv);
+    m.part_bytes = 2 * (size_t)m.wgs * (4 / m.kw) * (D / 8 + 1) * 1024;
+  }
   return m;
 }
 
@@ -95,7 +97,7 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
   m.max_blocks = g.max_blocks;
   m.scale_log2 = g.scale_log2;
   m.window = c.mask.window;
-  if (g.S <= 0 || !mfma_ok(m) || (long long)g.nb * g.bs * (m.kind == KvKind::affine ? g.Hkv : 1) >= (1LL << 31))
+  if (g.S <= 0 || g.S > kWideSeqs || !mfma_ok(m) || (long long)g.nb * g.bs * (m.kind == KvKind::affine ? g.Hkv : 1) >= (1LL << 31))
     return false;
   const size_t base = workspace_base();
   // rows of one token: the split-K decode (a tile of the kernel below would hold a group's heads alone)
@@ -109,9 +111,11 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
   }
   MaskedShape shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, true);
   if (shape.tokb == 0) return false;
-  if (shape.part_bytes && (!c.ws || c.ws_bytes < base + shape.part_bytes))
+  // (the blocks of a cut launch are counted in 31 bits)
+  if (shape.wgs && (!c.ws || c.ws_bytes < base + shape.desc_bytes + shape.part_bytes ||
+                    (double)shape.tiles * g.Hkv * ((double)g.max_blocks * g.bs / 32 + 2) >= 2147483648.0))
     shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, false);
-  if (shape.units * g.Hkv >= (1L << 31)) return false;
+  if (shape.tiles * g.Hkv >= (1L << 31)) return false;
   MaskedArgs a{};
   a.d.q = static_cast<const h16*>(m.q);
   a.d.kc = static_cast<const uint32_t*>(m.k);
@@ -139,16 +143,19 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
   a.tokb = shape.tokb;
   a.T = m.T;
   a.tiles = (int)shape.tiles;
-  a.share_of = (int)shape.share_of;
-  a.units = (int)shape.units;
-  a.part = shape.part_bytes ? reinterpret_cast<float*>(static_cast<char*>(c.ws) + base) : nullptr;
-  switch (m.kind) {
-    case KvKind::f16: launch_masked_kind<KvF16>(a, m.D, shape.ct, c.st); break;
-    case KvKind::bf16: launch_masked_kind<KvBF16>(a, m.D, shape.ct, c.st); break;
-    case KvKind::fp8: launch_masked_kind<KvFp8>(a, m.D, shape.ct, c.st); break;
-    case KvKind::affine: launch_masked_affine(m, a, shape.ct, c.st); break;
+  a.wgs = shape.wgs;
+  if (a.wgs) {
+    char* p = static_cast<char*>(c.ws) + base;
+    a.part = reinterpret_cast<float*>(p);
+    a.desc = reinterpret_cast<int4*>(p + shape.part_bytes);
   }
-  *rc = entry_check_launch("masked_mfma");
+  switch (m.kind) {
+    case KvKind::f16: launch_masked_kind<KvF16>(a, m.D, shape.kw, c.st); break;
+    case KvKind::bf16: launch_masked_kind<KvBF16>(a, m.D, shape.kw, c.st); break;
+    case KvKind::fp8: launch_masked_kind<KvFp8>(a, m.D, shape.kw, c.st); break;
+    case KvKind::affine: launch_masked_affine(m, a, shape.kw, c.st); break;
+  }
+  *rc = entry_check_launch("masked_wide");
   return true;
 }
 
@@ -163,7 +170,8 @@ size_t emx_masked_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads,
   if (num_tokens <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       !head_ok(head_dim))
     return 0;
-  size_t part = masked_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, true).part_bytes;
+  const MaskedShape m = masked_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, true);
+  size_t part = m.desc_bytes + m.part_bytes;
   if (num_tokens == num_seqs)
     part = std::max(part, decode_mfma_partial_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim));
   return part ? workspace_base() + part : 0;

@@ -1,5 +1,5 @@
 // Masked paged attention (masked_launch.hpp) for any head_dim <= 256, page size and cache type:
-// the shapes outside masked_mfma.hpp, fp32 among them.
+// the shapes outside masked_wide.hpp, fp32 among them.
 //
 // One wavefront per (token, kv_head, up to 16 query heads), keys 64 at a time: a key to a lane
 // for the scores (with the lane's own walk up the tree where the block holds drafted nodes), then

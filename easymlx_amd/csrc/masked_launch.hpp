@@ -56,20 +56,20 @@ __device__ __forceinline__ int node_depth(const int32_t* par, int i) {
   return d;
 }
 
-struct MaskedArgs;  // masked_mfma.hpp
+struct MaskedArgs;  // masked_wide.hpp
 
-// How a call is cut (sizes and types only): columns of a wave / 16, query tokens of a tile, the most tiles per kv
-// head, over how many units per kv head its blocks are spread (0: tiles are not cut) and the units the grid has room for.
+// How a call is cut (sizes and types only).
 struct MaskedShape {
-  int ct, tokb;
-  long tiles, share_of, units;
-  size_t part_bytes;  // of all units
+  int kw, tokb;       // key waves of a workgroup, query tokens of a tile (0: not taken)
+  long tiles;         // the most tiles per kv head
+  int wgs;            // workgroups over which tiles are cut, 0: they are not
+  size_t desc_bytes, part_bytes;
 };
 MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, bool cut);
 
 // Single-token rows (c.qsl null) with a window and sinks > 0; buffers as launch_decode_mfma's (emx_masked_rows.hip).
 void launch_masked_rows(const MfmaCall& c, int sinks, int* ws_cnt, float* partials, hipStream_t st);
 
-void launch_masked_affine(const MfmaCall& c, const MaskedArgs& a, int ct, hipStream_t st);  // emx_masked_affine.hip
+void launch_masked_affine(const MfmaCall& c, const MaskedArgs& a, int kw, hipStream_t st);  // emx_masked_affine.hip
 
 }  // namespace emx

@@ -1,0 +1,1136 @@
+// Masked paged attention (masked_launch.hpp: sliding windows with sinks, drafted trees) on the
+// matrix units: head_dim 64, 128 or 256, any GQA ratio up to the columns of a tile, over
+// token-major caches [nb, bs, Hkv, D] (fp16 / bf16, FP8 E4M3 with one fp32 scale per page; pages
+// of a multiple of 8 tokens) and over affine pages.
+//
+//   O_i = sum_k p_ik V_k / sum_k p_ik,  p_ik = 2^(scale log2(e) q_i . K_k - m_i) over the keys k
+//   that row i sees,
+//
+// in one pass over the keys with the running reference m_i.
+//
+// Work: a tile is the 32 CW query columns (token, head), head fastest, of COLS / HG tokens of one
+// sequence and kv head; its keys go in blocks of NT positions, from the last backwards and then the
+// sinks' blocks: those between the sinks and the earliest window are not read.  From the last
+// backwards because a drafted node's ancestors then come in the order of its walk to the root: each
+// lane keeps one cursor, and a block of drafted keys costs as many steps as it holds ancestors, for
+// trees of any size.  Where a launch has tiles enough each is a workgroup's; else the blocks of all
+// tiles in a row are cut into equal ranges, one to a workgroup (WidePlan), and a tile that is not
+// inside one range leaves its parts' fp32 state to masked_merge, which joins them in part order.
+//
+// A block: K and V are loaded once per workgroup, a block ahead into registers, and go to the other
+// of two LDS images as 16-bit values (FP8: dec(code) * 2^-8, exact; affine codes as exact
+// sub-normals), 16-byte chunks turned by the row so that operand reads touch every bank: one barrier
+// a block.  A wave has 32 columns (and, KW = 2, half of the block's keys), on v_mfma 32x32x16:
+//   S^T : A = K rows, B = queries; a lane ends with half of its tile's scores of ONE column, so that
+//         maximum, reference and sum are its own, and lanes meet only where a score passes the
+//         reference by 2^kLazyMax;
+//   O^T += V^T P^T : A = V^T by the transposing LDS read (affine values lie dim-major already), B = the
+//         lane's own probabilities as two 16-bit parts, each the nearest (fp16: 22 bits of the 24; bf16:
+//         16, which puts an output off by at most 2^-17 of the largest value it averages: one part would
+//         add an error as large as the output's own rounding).
+#pragma once
+
+#include "masked_launch.hpp"
+#include "prefill_mfma.hpp"
+
+namespace emx {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(const h16x8 a, const h16x8 b, const f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(const bf16x8 a, const bf16x8 b, const f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ void split_p2(const float (&x)[8], h16x8 (&p)[2]) { split_p(x, p); }
+__device__ __forceinline__ void split_p2(const float (&x)[8], bf16x8 (&p)[2]) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  typedef float f32x2v __attribute__((ext_vector_type(2)));
+  uint32_t w[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t h =
+        __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2v{x[2 * i], x[2 * i + 1]}, bf16x2));
+    w[0][i] = h;
+    w[1][i] = __builtin_bit_cast(
+        uint32_t, __builtin_convertvector(f32x2v{x[2 * i] - __uint_as_float(h << 16),
+                                                 x[2 * i + 1] - __uint_as_float(h & 0xFFFF0000u)},
+                                          bf16x2));
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) p[k] = __builtin_bit_cast(bf16x8, u32x4{w[k][0], w[k][1], w[k][2], w[k][3]});
+}
+
+struct MaskedArgs {
+  DecodeArgs d;     // kc / vc: the caches; qsl null: token i is sequence i
+  MaskRule mask;
+  uint32_t inv_bs;  // ceil(2^32 / bs)
+  int tokb;         // query tokens per tile: columns / HG
+  int T;            // query rows
+  int tiles;        // tiles per kv head, at most
+  int wgs;          // > 0: tiles are cut, over at most that many workgroups; 0: a workgroup to a tile
+  int4* desc;       // cut: [1 + Hkv * tiles] {tiles of the launch}, then what masked_merge has to know of a tile
+  float* part;      // cut: [2 * wgs][part floats]
+};
+
+// Fewest blocks of a workgroup's range; and how many blocks longer than an equal share the longest tile may be before
+// tiles are cut, where there is a workgroup for each (parts go to memory and back: 64 KiB each way, and a launch).
+constexpr int kWideRangeBlocks = 2;
+constexpr int kWideCutBlocks = 6;
+constexpr int kWideTreeLds = 512;  // nodes of a tree whose parents are kept in LDS
+
+template <class C, int D, int KW>
+struct WideCfg {
+  static constexpr int EB = sizeof(typename C::ET);
+  static constexpr int CW = 4 / KW;                 // waves side by side over the columns
+  static constexpr int COLS = 32 * CW;
+  static constexpr int NT = D > 128 ? 32 * KW : 64; // keys of a block
+  static constexpr int KT = NT / KW / 32;           // 32-key tiles of a wave's share of it
+  static constexpr int KS = D / 16;                 // QK^T k-slices
+  static constexpr int DT = D / 32;                 // PV dim tiles
+  static constexpr int G = 1;
+  static constexpr int PR = D * EB / 16;            // 16-byte pieces per row
+  static constexpr int NP = NT * PR / 256;          // pieces per thread and block, of K and of V
+  static constexpr int VB = NT * D * 2;             // bytes of the V image
+  static constexpr int SCB = C::kFp8 ? 2 * 4 * NT : 0;  // of the scales
+  static_assert(KT >= 1 && NT * PR % 256 == 0, "whole 32-key tiles and pieces");
+};
+template <int BITS, int GS, int D, int KW>
+struct WideCfg<KvAffine<BITS, GS>, D, KW> {
+  static constexpr int CW = 4 / KW, COLS = 32 * CW, NT = D > 128 ? 32 * KW : 64, KT = NT / KW / 32;
+  static constexpr int KS = D / 16, DT = D / 32, G = D / GS;
+  static constexpr int RBK = D * BITS / 8;              // bytes of a key's codes
+  static constexpr int PR = RBK / 16;                   // 16-byte pieces of them
+  static constexpr int NPK = NT * PR;                   // K pieces of a block
+  static constexpr int NP = (NPK + 255) / 256;
+  static constexpr int UT = 64 / BITS, U = NT / UT;     // V units: 8 bytes, UT tokens of one dim
+  static constexpr int NPV = D * U / 256;               // V units per thread
+  static constexpr int NPS = 4 * G * NT / 8;            // 16-byte scale pieces of a block
+  static constexpr int VB = D * NT * 2;                 // [dim][NT], 16-byte chunks turned by v_turn
+  static constexpr int SCB = 3 * 4 * G * NT + 16 * NT;  // ks, vs, vb [group][NT] floats, bias operand rows
+  static_assert(NPS <= 64 && D * U % 256 == 0, "one scale piece per lane, whole V units per thread");
+};
+
+// Where 16-byte chunk c of a row stands in its row, so that the lanes that LDS serves in one cycle touch all 64 banks.
+// K: 16 rows at one chunk; token-major V: 4 rows at 4 neighbouring chunks; affine V (a row: NT keys of a dim): 16 rows
+// at one chunk.  Each turns with the row alone, so that an operand's address is a lane's, with constant bits flipped.
+// (With every row turned by its low three bits alone more than half of the LDS cycles were conflicts.)
+template <int D>
+__device__ __forceinline__ constexpr int k_turn(const int row, const int c) {
+  return c ^ (D == 64 ? (row >> 1) & 7 : row & 15);
+}
+template <int D>
+__device__ __forceinline__ constexpr int v_turn(const int row, const int c) {
+  return c ^ (D == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2);
+}
+template <int NT>
+__device__ __forceinline__ constexpr int va_turn(const int dim, const int c) {
+  return c ^ (NT == 64 ? (dim >> 1) & 7 : (dim >> 2) & 3);
+}
+
+// Floats of a part: per column wave DT * 4 + 1 vectors of 4 a lane.
+template <int D, int KW>
+constexpr int kWidePart = (4 / KW) * (D / 8 + 1) * 256;
+
+// A tile's blocks: positions backwards from block `hi`, `n` in all, the last `sink` of them the blocks 0 .. sink - 1.
+struct MaskedSpan {
+  int hi, n, sink;
+};
+
+template <int NT>
+__device__ __forceinline__ MaskedSpan masked_span(const MaskRule& m, const int past, const int tok_lo,
+                                                  const int tok_hi) {
+  MaskedSpan r{0, 0, 0};
+  const int k_hi = past + tok_hi;
+  if (k_hi < 0) return r;
+  // the earliest first key of the tile's windows (a node's place is at least its tree's start); a
+  // tree's own keys stand at places below their positions, and are all read
+  int first = 0;
+  if (m.window > 0) first = max(0, (m.parents ? past : past + tok_lo) - m.window + 1);
+  if (m.parents) first = min(first, max(past, 0));
+  r.hi = k_hi / NT;
+  const int lo = min(first, k_hi) / NT;
+  r.sink = min((min(m.sinks, k_hi + 1) + NT - 1) / NT, lo);
+  r.n = r.hi - lo + 1 + r.sink;
+  return r;
+}
+
+struct MaskedSeq {
+  int s, q0, qlen, past;
+};
+
+__device__ __forceinline__ MaskedSeq masked_seq(const MaskedArgs& A, const int s) {
+  const DecodeArgs& a = A.d;
+  MaskedSeq r;
+  r.s = s;
+  r.q0 = a.qsl ? a.qsl[s] : s;
+  r.qlen = a.qsl ? (r.q0 < 0 ? 0 : max(a.qsl[s + 1] - r.q0, 0)) : 1;
+  r.past = min(max(a.kv_lens[s], 0), a.max_blocks * a.bs) - r.qlen;
+  return r;
+}
+
+// Last token of tile `tile` of the sequence (rows past the call's are no tokens).
+__device__ __forceinline__ int masked_tok_hi(const MaskedArgs& A, const MaskedSeq& q, const int tile) {
+  return min(min((tile + 1) * A.tokb, q.qlen), A.T - q.q0) - 1;
+}
+
+// Blocks of a tile, at least one (an empty one writes its rows' zeros).
+template <int NT>
+__device__ __forceinline__ int masked_blocks(const MaskedArgs& A, const MaskedSeq& q, const int tile) {
+  return max(1, masked_span<NT>(A.mask, q.past, tile * A.tokb, masked_tok_hi(A, q, tile)).n);
+}
+
+// The sum over the workgroup of the threads before this one (256 threads; red: 8 ints of LDS); total: of all.
+__device__ __forceinline__ int wg_scan(const int mine, int* red, int& total) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int x = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int y = __shfl_up(x, o, 64);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();  // (red may still be read)
+  if (lane == 63) red[wv] = x;
+  __syncthreads();
+  int base = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    base += w < wv ? red[w] : 0;
+    total += red[w];
+  }
+  return base + x - mine;
+}
+
+constexpr int kWideSeqs = 1024;   // sequences of a call
+constexpr int kWideSeqLds = 256;  // sequences whose place and lengths are kept in LDS
+
+// Sequence s as wide_tiles left it in LDS (a call of more sequences: from memory).
+__device__ __forceinline__ MaskedSeq wide_seq(const MaskedArgs& A, const int* seqs, const int s) {
+  if (A.d.S > kWideSeqLds) return masked_seq(A, s);
+  return MaskedSeq{s, seqs[s], seqs[kWideSeqLds + s], seqs[2 * kWideSeqLds + s]};
+}
+
+// tcum[s]: tiles of the sequences before s, tcum[S] of all; seqs: wide_seq's.
+__device__ __forceinline__ void wide_tiles(const MaskedArgs& A, int* tcum, int* seqs, int* red) {
+  const int S = A.d.S, ch = (S + 255) / 256, s0 = threadIdx.x * ch;
+  int mine = 0, total;
+  for (int i = 0; i < ch && s0 + i < S; ++i) {
+    const MaskedSeq q = masked_seq(A, s0 + i);
+    const int n = (q.qlen + A.tokb - 1) / A.tokb;
+    tcum[s0 + i] = n;
+    mine += n;
+    if (S <= kWideSeqLds) {
+      seqs[s0 + i] = q.q0;
+      seqs[kWideSeqLds + s0 + i] = q.qlen;
+      seqs[2 * kWideSeqLds + s0 + i] = q.past;
+    }
+  }
+  int run = wg_scan(mine, red, total);
+  for (int i = 0; i < ch && s0 + i < S; ++i) {
+    const int n = tcum[s0 + i];
+    tcum[s0 + i] = run;
+    run += n;
+  }
+  if (threadIdx.x == 0) tcum[S] = total;
+  __syncthreads();
+}
+
+// The sequence of tile t: the largest s with tcum[s] <= t (t < tcum[S]).
+__device__ __forceinline__ int wide_seq_of(const int* tcum, const int S, const int t) {
+  int lo = 0, hi = S;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tcum[mid] <= t) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// One query row in fp32 on one wave over every key that it sees: rows whose result on the matrix unit is not
+// finite are computed again here, dims [d0, d1) of them (there a key that the row does not see still enters its tile's product with p = 0,
+// and 0 * inf makes NaN of what these rules leave alone).  64 keys at a time, as attend_row (mfma_common.hpp).
+template <class C, int D>
+__device__ void attend_masked(const DecodeArgs& a, const MaskRule& mask, const MaskedSeq& sq, const int kvh, const int i,
+                              const int hd, const int lane, const int d0 = 0, const int d1 = D) {
+  constexpr int N = D / 64;
+  typedef typename C::QT QT;
+  const auto kv = kv_loader<C>(a, D);
+  const int32_t* par = mask.parents ? mask.parents + sq.q0 : nullptr;
+  const int depth = par && mask.window > 0 ? node_depth(par, i) : 0;
+  const size_t ro = ((size_t)(sq.q0 + i) * a.Hq + (size_t)kvh * (a.Hq / a.Hkv) + hd) * D;
+  const QT* q = reinterpret_cast<const QT*>(a.q) + ro;
+  float qv[N], acc[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    qv[n] = to_f32(q[lane + 64 * n]);
+    acc[n] = 0.f;
+  }
+#pragma unroll 1
+  for (int base = 0; base <= sq.past + i; base += 64) {
+    const int k = base + lane;
+    const bool see = k <= sq.past + i && key_visible(mask, par, sq.past, i, depth, k);
+    const int blk = see ? a.block_tables[(size_t)sq.s * a.max_blocks + k / a.bs] : -1;
+    const bool ok = (unsigned)blk < (unsigned)a.nb;
+    const uint64_t okm = __ballot(ok);
+    if (!okm) continue;
+    float x = 0.f;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll 1
+      for (int d = 0; d < 64; d += 32) {
+        float kd[32] = {};
+        if (ok) key32(kv, blk, k % a.bs, kvh, 64 * n + d, kd);
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          x = fmaf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(qv[n]), d + j)), kd[j], x);
+      }
+    x = ok ? x * a.scale_log2 : -INFINITY;
+    const float mn = fmaxf(m, wave_max(x));
+    const float p = ok && (mn != -INFINITY || x != x) ? exp2f(x - mn) : 0.f;
+    const float al = m == mn ? 1.f : exp2f(m - mn);
+    l = l * al + wave_sum(p);
+    m = mn;
+#pragma unroll
+    for (int n = 0; n < N; ++n) acc[n] *= al;
+#pragma unroll 1
+    for (int t = 0; t < 64; t += 8) {
+      const uint32_t live = (uint32_t)(okm >> t) & 0xFFu;
+      if (!live) continue;
+      const int b = __builtin_amdgcn_readlane(blk, t + __builtin_ctz(live));
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        float v[8];
+        val8(kv, b, (base + t) % a.bs, kvh, lane + 64 * n, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float pj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), t + j));
+          acc[n] = (live >> j) & 1u ? fmaf(pj, v[j], acc[n]) : acc[n];
+        }
+      }
+    }
+  }
+  const float li = l > 0.f || l != l ? 1.f / l : 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    if (lane + 64 * n >= d0 && lane + 64 * n < d1) from_f32(acc[n] * li, reinterpret_cast<QT*>(a.out) + ro + lane + 64 * n);
+}
+
+// Column c of a tile: which token and head; token -1 where there is none.
+__device__ __forceinline__ void masked_column(const MaskedArgs& A, const MaskedSeq& q, const int tile, const int c,
+                                              const int HG, int& tok, int& head) {
+  const int t = c / HG;
+  tok = tile * A.tokb + t;
+  head = c - t * HG;
+  if (t >= A.tokb || tok >= q.qlen || (unsigned)(q.q0 + tok) >= (unsigned)A.T) tok = -1;
+}
+
+// Four dims from `dim` of a column, normalised and written.  True where a value is not finite.
+template <class C, int D>
+__device__ __forceinline__ bool masked_write(const DecodeArgs& a, const MaskedSeq& q, const int kvh, const int tok,
+                                             const int head, const f32x4 o, const float l, const float inv,
+                                             const int dim) {
+  typedef typename C::QT QT;
+  struct alignas(8) Four {
+    QT x[4];
+  } v;
+  bool bad = not_finite(l);
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    bad = bad || not_finite(o[r]);
+    from_f32(o[r] * inv, &v.x[r]);
+  }
+  if (tok >= 0)
+    *reinterpret_cast<Four*>(reinterpret_cast<QT*>(a.out) +
+                             ((size_t)(q.q0 + tok) * a.Hq + (size_t)kvh * (a.Hq / a.Hkv) + head) * D + dim) = v;
+  return bad && tok >= 0;
+}
+
+// The lowest n of 32 bits (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(const int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
+}
+
+// (Two workgroups to a compute unit where a wave's state fits 256 registers.)
+template <class C, int D, int KW>
+__global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 1)) ? 1 : 2) void masked_wide(MaskedArgs A) {
+  using P = WideCfg<C, D, KW>;
+  typedef typename C::Op Op;
+  typedef typename C::QT QT;
+  const DecodeArgs& a = A.d;
+  constexpr int NT = P::NT, KT = P::KT, KS = P::KS, DT = P::DT, G = P::G, CW = P::CW;
+  constexpr bool AFF = C::kAffine, FP8 = C::kFp8;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cw = wv % CW, kw = wv / CW;  // this wave's columns, and its share of a block's keys
+  const int c32 = lane & 31, half = lane >> 5;
+
+  // ---- LDS: tables, then two images of a block (K rows, V, scales); the states of a unit's key waves meet there too
+  constexpr int oTc = 0, oSeq = lds_next(oTc, 4 * (kWideSeqs + 1));
+  constexpr int oPar = lds_next(oSeq, 12 * kWideSeqLds), oRed = lds_next(oPar, 4 * kWideTreeLds);
+  constexpr int oBuf = (lds_next(oRed, 128) + 511) & ~511;
+  constexpr int KB = NT * D * 2, oV = KB, oSc = oV + P::VB, BUF = (oSc + P::SCB + 16 + 511) & ~511;
+  static_assert(KB % 512 == 0 && P::VB % 512 == 0, "the images' chunks are flipped by address bits");
+  constexpr int MEET = KW > 1 ? CW * (4 * DT + 1) * 64 * 16 : 0;
+  constexpr int oEnd = oBuf + (2 * BUF > MEET ? 2 * BUF : MEET);
+  static_assert(oEnd <= 81920, "two workgroups to a compute unit");
+  __shared__ __attribute__((aligned(512))) unsigned char lds[oEnd];
+  int* tcum = reinterpret_cast<int*>(lds + oTc);
+  int* seqs = reinterpret_cast<int*>(lds + oSeq);
+  int* lpar = reinterpret_cast<int*>(lds + oPar);
+  int* red = reinterpret_cast<int*>(lds + oRed);
+
+  const MaskRule mask = A.mask;
+  const int HG = a.Hq / a.Hkv, S = a.S;
+  if (a.qsl) {
+    const int lo = a.qsl[0], hi = a.qsl[S];
+    if (lo > 0 || hi < A.T) zero_other_rows<QT>(a, A.T, D, blockIdx.x, gridDim.x);
+  }
+
+  // ---- this workgroup's range [at, end) of the blocks of all tiles, kv head by kv head
+  wide_tiles(A, tcum, seqs, red);
+  const int ntiles = __builtin_amdgcn_readfirstlane(tcum[S]);
+  int kvh, t, b0, todo, w = 0, nwg = 0, all = 0;  // kv head, tile, block within it, blocks left; nwg 0: no tile is cut
+  if (A.wgs == 0) {
+    kvh = blockIdx.x % a.Hkv;
+    t = ntiles - 1 - (int)blockIdx.x / a.Hkv;  // (the longest of a sequence first)
+    b0 = 0;
+    todo = 0x7FFFFFFF;
+    if (t < 0) return;
+  } else {
+    const int ch = (ntiles + 255) / 256, t0 = tid * ch;
+    int mine = 0, most = 0, per;
+    for (int i = 0, s = 0; i < ch && t0 + i < ntiles; ++i) {
+      if (i == 0) s = wide_seq_of(tcum, S, t0);
+      while (tcum[s + 1] <= t0 + i) ++s;
+      const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]);
+      mine += n;
+      most = max(most, n);
+    }
+    most = (int)wave_max((float)most);
+    if (lane == 0) red[4 + wv] = most;
+    const int before = wg_scan(mine, red, per);
+    most = max(max(red[4], red[5]), max(red[6], red[7]));
+    all = per * a.Hkv;  // (the host keeps it below 2^31)
+    nwg = min(A.wgs, max(1, all / kWideRangeBlocks));
+    if (nwg >= 8) nwg &= ~7;
+    const int nt = ntiles * a.Hkv;
+    if (nt <= A.wgs && most <= all / nwg + kWideCutBlocks) {  // a tile to a workgroup
+      nwg = 0;
+      if (blockIdx.x == 0 && tid == 0) A.desc[0] = int4{0, 0, 0, 0};
+      if ((int)blockIdx.x >= nt) return;
+      kvh = blockIdx.x % a.Hkv;
+      t = blockIdx.x / a.Hkv;
+      b0 = 0;
+      todo = 0x7FFFFFFF;
+    } else {
+    if ((int)blockIdx.x >= nwg) return;
+    // workgroups of one XCD (blockIdx mod 8) take neighbouring ranges: tiles of one sequence and kv head share its L2
+    w = nwg >= 8 ? (int)(blockIdx.x % 8) * (nwg / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+    const int at = (int)((long long)w * all / nwg);
+    todo = (int)((long long)(w + 1) * all / nwg) - at;
+    kvh = at / per;
+    const int r = at - kvh * per;
+    if (r >= before && r < before + mine) {  // one thread's tiles hold it
+      int x = before, i = 0, s = wide_seq_of(tcum, S, t0);
+      for (;; ++i) {
+        while (tcum[s + 1] <= t0 + i) ++s;
+        const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]);
+        if (r < x + n) break;
+        x += n;
+      }
+      red[8] = t0 + i;
+      red[9] = r - x;
+    }
+    if (blockIdx.x == 0 && tid == 0) A.desc[0] = int4{ntiles, 0, 0, 0};
+    __syncthreads();
+    t = __builtin_amdgcn_readfirstlane(red[8]);
+    b0 = __builtin_amdgcn_readfirstlane(red[9]);
+    }
+  }
+
+  // ---- lane constants of the operand reads (image-relative bytes; the images start at multiples of 512)
+  const int kad = (kw * KT * 32 + c32) * (D * 2) + (k_turn<D>(c32, half) << 4);  // K: row c32 (+ 32 per tile), chunk 2 w + half
+  int vad;  // V: 4 tokens of 16 dims per 16 lanes, chunk 4 d + ..; affine: dim c32 (+ 32 per tile), chunk 4 kt + 2 j + half
+  if constexpr (AFF) {
+    vad = oV + c32 * (NT * 2) + (va_turn<NT>(c32, kw * KT * 4 + half) << 4);
+  } else {
+    const int i = lane & 15, row = 4 * half + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+    vad = oV + (kw * KT * 32 + row) * (D * 2) + (v_turn<D>(row, c) << 4) + (i & 1) * 8;
+  }
+  const float sl2 = a.scale_log2;
+  const size_t rowb = (size_t)a.Hkv * D * sizeof(typename C::ET);  // token-major
+  typedef __attribute__((address_space(3))) unsigned char* lptr;
+
+  bool first_seg = true;
+  int sidx = wide_seq_of(tcum, S, t);
+  for (;;) {
+    // ---- a segment: blocks [b0, b1) of tile t
+    while (tcum[sidx + 1] <= t) ++sidx;
+    MaskedSeq sq = wide_seq(A, seqs, __builtin_amdgcn_readfirstlane(sidx));
+    sq.q0 = __builtin_amdgcn_readfirstlane(sq.q0);
+    sq.qlen = __builtin_amdgcn_readfirstlane(sq.qlen);
+    sq.past = __builtin_amdgcn_readfirstlane(sq.past);
+    const int tile = t - __builtin_amdgcn_readfirstlane(tcum[sidx]);
+    const int q0 = sq.q0, past = sq.past;
+    const int tok_lo = tile * A.tokb, tok_hi = masked_tok_hi(A, sq, tile);
+    const MaskedSpan span = masked_span<NT>(mask, past, tok_lo, tok_hi);
+    const int nblk = max(1, span.n), b1 = min(nblk, b0 + min(todo, nblk - b0));
+    const int st_lo = b0, st_hi = min(b1, span.n);  // (an empty tile has a block of nothing)
+    const int k_hi = max(past + tok_hi, 0);
+    const int32_t* par = mask.parents ? mask.parents + q0 : nullptr;
+    const bool tree = par != nullptr, tree_lds = tree && sq.qlen <= kWideTreeLds;
+    __syncthreads();  // (the last segment's LDS is free)
+    if (tree_lds) {
+      for (int i = tid; i <= tok_hi; i += 256) lpar[i] = parent_of(par, i);
+      __syncthreads();
+    }
+    auto up = [&](const int i) { return tree_lds ? lpar[i] : parent_of(par, i); };
+    auto pos_of_block = [&](const int st) {
+      const int lo = span.n - span.sink;
+      return (st < lo ? span.hi - st : span.sink - 1 - (st - lo)) * NT;
+    };
+
+    // ---- pages: lane l holds the page id of key l of a block (positions past the tile's last key repeat it)
+    const char* kbase = reinterpret_cast<const char*>(a.kc) + (AFF ? 0 : (size_t)kvh * (D * sizeof(typename C::ET)));
+    const char* vbase = reinterpret_cast<const char*>(a.vc) + (AFF ? 0 : (size_t)kvh * (D * sizeof(typename C::ET)));
+    const int32_t* bt = a.block_tables + (size_t)sq.s * a.max_blocks;
+    auto page_id = [&](const int st) {
+      return bt[page_of(min(pos_of_block(st) + (lane & (NT - 1)), k_hi), A.inv_bs)];
+    };
+    u32x4 rk[P::NP], rv[AFF ? 1 : P::NP];  // the next block's pieces
+    u32x2 ru[AFF ? 16 : 1];                // affine: its V units
+    u32x4 rs;                              // affine, wave 0: scale piece `lane`
+    uint64_t okn = 0;                      // keys of that block on a valid page
+    float psk = 0.f, psv = 0.f;            // FP8: page scales of key `lane` of that block
+    auto load_block = [&](const int st, const int blk) {
+      const int pos = min(pos_of_block(st) + (lane & (NT - 1)), k_hi);
+      const bool ok = (unsigned)blk < (unsigned)a.nb;
+      okn = __ballot(ok);
+      const int b = ok ? blk : 0;
+      const int off = pos - page_of(pos, A.inv_bs) * a.bs;
+      if constexpr (AFF) {
+        constexpr int B = C::kBits;
+        const int row = (b * a.Hkv + kvh) * a.bs + off;
+        if (wv == 0) {
+          const int pc = min(lane, P::NPS - 1), seg = pc / (NT / 8), arr = seg / G, g = seg % G;
+          const int r8 = __shfl(row, 8 * (pc % (NT / 8)), 64), o8 = __shfl(off, 8 * (pc % (NT / 8)), 64);
+          const h16 *b_ks = a.ks, *b_kb = a.kb, *b_vs = a.vs, *b_vb = a.vb;
+          asm("" : "+s"(b_ks), "+s"(b_kb), "+s"(b_vs), "+s"(b_vb));  // picked from registers, not by a vector load
+          const h16* base = arr == 0 ? b_ks : arr == 1 ? b_kb : arr == 2 ? b_vs : b_vb;
+          typedef const __attribute__((address_space(1))) u32x4* gu32x4;
+          // (past the tile's last key the group's first token may repeat it: aligned down, inside the page)
+          rs = *(gu32x4)(base + (size_t)G * (r8 - o8) + (size_t)g * a.bs + (o8 & ~7));
+        }
+#pragma unroll
+        for (int n = 0; n < P::NP; ++n) {
+          const int e = tid + 256 * n;  // (fewer than 256 pieces: the others repeat them)
+          const int r = __shfl(row, (e / P::PR) & (NT - 1), 64);
+          rk[n] = *reinterpret_cast<const u32x4*>(kbase + (size_t)r * P::RBK + 16 * (e % P::PR));
+        }
+        const int T = min(a.bs, 256 / B);  // tokens of a value tile (a power of two)
+#pragma unroll
+        for (int n = 0; n < P::NPV; ++n) {
+          const int e = tid + 256 * n, uu = e % P::U, dim = e / P::U;
+          const int r = __shfl(row, uu * P::UT, 64);
+          const int o = (r & (T - 1)) & ~(P::UT - 1);
+          ru[n] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint32_t*>(vbase) +
+                                                  (size_t)(r & ~(T - 1)) * (D * B / 32) + (dim * T + o) * B / 32);
+        }
+      } else {
+        const int row = b * a.bs + off;
+        if constexpr (FP8) {
+          psk = a.kps[b];
+          psv = a.vps[b];
+        }
+#pragma unroll
+        for (int n = 0; n < P::NP; ++n) {
+          const size_t o = (size_t)__shfl(row, tid / P::PR + n * (256 / P::PR), 64) * rowb + 16 * (tid % P::PR);
+          rk[n] = *reinterpret_cast<const u32x4*>(kbase + o);
+          rv[n] = *reinterpret_cast<const u32x4*>(vbase + o);
+        }
+      }
+    };
+    // ... and their way to image `buf`, once they are here.  vex: the exponent that the value scales of the images carry
+    int vex = 0;
+    auto store_block = [&](const int st, const int buf) {
+      unsigned char* img = lds + oBuf + buf * BUF;
+      if constexpr (AFF) {
+        constexpr int B = C::kBits;
+#pragma unroll
+        for (int n = 0; n < P::NP; ++n) {
+          const int e = tid + 256 * n, row = (e / P::PR) & (NT - 1), c0 = (e % P::PR) * (16 / B);
+          unsigned char* kr = img + row * (D * 2);
+          if (e < P::NPK) {
+            if constexpr (B == 4) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<h16x8*>(kr + (k_turn<D>(row, c0 + i) << 4)) = unpack4_high(rk[n][i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<h16x8*>(kr + (k_turn<D>(row, c0 + i) << 4)) = unpack8(rk[n][2 * i], rk[n][2 * i + 1]);
+            }
+          }
+        }
+        // values: a dim's 16 tokens stand as 0-3, 8-11 and 4-7, 12-15: one read has a lane's eight
+#pragma unroll
+        for (int n = 0; n < P::NPV; ++n) {
+          const int e = tid + 256 * n, dim = e / P::U, uu = e % P::U;
+          unsigned char* vr = img + oV + dim * (NT * 2);
+          if constexpr (B == 4) {
+            const u32x4 x = __builtin_bit_cast(u32x4, unpack4_high(ru[n][0]));
+            const u32x4 y = __builtin_bit_cast(u32x4, unpack4_high(ru[n][1]));
+            *reinterpret_cast<u32x4*>(vr + 16 * va_turn<NT>(dim, 2 * uu)) = u32x4{x[0], x[1], y[0], y[1]};
+            *reinterpret_cast<u32x4*>(vr + 16 * va_turn<NT>(dim, 2 * uu + 1)) = u32x4{x[2], x[3], y[2], y[3]};
+          } else {  // (a unit is the first or the second half of its 16)
+            const u32x4 x = __builtin_bit_cast(u32x4, unpack8(ru[n][0], ru[n][1]));
+            const int c = uu & ~1, h8 = 8 * (uu & 1);
+            *reinterpret_cast<u32x2*>(vr + 16 * va_turn<NT>(dim, c) + h8) = u32x2{x[0], x[1]};
+            *reinterpret_cast<u32x2*>(vr + 16 * va_turn<NT>(dim, c + 1) + h8) = u32x2{x[2], x[3]};
+          }
+        }
+        if (wv == 0) {
+          float* ksf = reinterpret_cast<float*>(img + oSc);
+          float *vsf = ksf + G * NT, *vbf = vsf + G * NT;
+          h16* kbe = reinterpret_cast<h16*>(vbf + G * NT);
+          // scales of keys past the tile's last one or on an invalid page (which may hold anything) as zeros
+          const int pc = min(lane, P::NPS - 1), t8 = 8 * (pc % (NT / 8)), seg = pc / (NT / 8), arr = seg / G,
+                    g = seg % G;
+          const int live = k_hi + 1 - pos_of_block(st) - t8;
+          u32x4 x = rs;
+          if (live < 8 || !((okn >> t8) & 1)) {
+            const int n = (okn >> t8) & 1 ? live : 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] &= (2 * e < n ? 0x0000FFFFu : 0u) | (2 * e + 1 < n ? 0xFFFF0000u : 0u);
+          }
+          int vm = 0;  // largest |v_scale|, as fp16 bits
+          if (arr == 2) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vm = max(vm, (int)max(x[e] & 0x7FFFu, (x[e] >> 16) & 0x7FFFu));
+          }
+          // the accumulator's exponent follows the value scales' (exact powers of two; 6 binades of slack)
+          const int ex = ((int)wave_max((float)vm) >> 10) - 15;
+          if (ex > vex || ex < vex - 6) vex = ex;
+          if (lane == 0) *reinterpret_cast<int*>(img + oSc + P::SCB) = vex;
+          if (lane < P::NPS) {
+            const float f = arr == 0   ? (float)(1 << C::kCodeExp)
+                            : arr == 2 ? __uint_as_float((uint32_t)(127 - vex) << 23)
+                                       : 1.f;
+            const h16x8 hv = __builtin_bit_cast(h16x8, x);
+            if (arr == 1) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) *reinterpret_cast<h16x2*>(kbe + 8 * (t8 + e) + 2 * g) = h16x2{hv[e], hv[e]};
+            } else {
+              float* dst = (arr == 0 ? ksf : arr == 2 ? vsf : vbf) + g * NT + t8;
+#pragma unroll
+              for (int q = 0; q < 2; ++q)
+                *reinterpret_cast<f32x4*>(dst + 4 * q) = f32x4{(float)hv[4 * q] * f, (float)hv[4 * q + 1] * f,
+                                                               (float)hv[4 * q + 2] * f, (float)hv[4 * q + 3] * f};
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < P::NP; ++n) {
+          const int row = tid / P::PR + n * (256 / P::PR), c = (tid % P::PR) * (16 / P::EB / 8);
+          unsigned char* kr = img + row * (D * 2);
+          unsigned char* vr = kr + oV;
+          if constexpr (FP8) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              auto wide8 = [&](const u32x4 x) {
+                return as_h8(e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e], 0x0C010C00u)),
+                             e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e], 0x0C030C02u)),
+                             e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e + 1], 0x0C010C00u)),
+                             e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e + 1], 0x0C030C02u)));
+              };
+              *reinterpret_cast<h16x8*>(kr + (k_turn<D>(row, c + e) << 4)) = wide8(rk[n]);
+              *reinterpret_cast<h16x8*>(vr + (v_turn<D>(row, c + e) << 4)) = wide8(rv[n]);
+            }
+          } else {
+            *reinterpret_cast<u32x4*>(kr + (k_turn<D>(row, c) << 4)) = rk[n];
+            *reinterpret_cast<u32x4*>(vr + (v_turn<D>(row, c) << 4)) = rv[n];
+          }
+        }
+        if constexpr (FP8) {
+          if (wv == 0) {
+            // value scales enter with the probabilities, brought near 1 by a power of two that the accumulator carries
+            const float vmax = wave_max(psv);
+            const int ex = min(max((int)((__float_as_uint(vmax) >> 23) & 0xFFu) - 127, -60), 60);
+            if (ex > vex || ex < vex - 6) vex = ex;
+            if (lane == 0) *reinterpret_cast<int*>(img + oSc + P::SCB) = vex;
+            float* ksf = reinterpret_cast<float*>(img + oSc);
+            if (lane < NT) {
+              ksf[lane] = psk * 256.f;
+              ksf[NT + lane] = psv * __uint_as_float((uint32_t)(127 - vex) << 23);
+            }
+          }
+        }
+      }
+    };
+
+    int blk1 = 0;
+    if (st_lo < st_hi) {
+      load_block(st_lo, page_id(st_lo));
+      blk1 = page_id(min(st_lo + 1, st_hi - 1));
+    }
+
+    // ---- this lane's column
+    int tok, head;
+    masked_column(A, sq, tile, cw * 32 + c32, HG, tok, head);
+    const bool busy = __any(tok >= 0);
+    int cur = tree ? tok : -1, back = 0;  // tree: the cursor, and how many steps above the column's node it is
+    int depth = 0;
+    if (tree && mask.window > 0)
+      for (int i = tok; i >= 0 && (i = up(i)) >= 0;) ++depth;
+    const int place = past + (tree ? depth : tok);
+    const int limit = tok < 0 ? -1 : tree ? past - 1 : place;  // last key of those outside the tree
+    const int start = mask.window > 0 ? max(0, place - mask.window + 1) : 0;
+    int lim_lo = tok >= 0 ? limit : 0x7FFFFFFF, start_hi = tok >= 0 ? start : 0;  // over the wave's columns
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      lim_lo = min(lim_lo, __shfl_xor(lim_lo, o, 64));
+      start_hi = max(start_hi, __shfl_xor(start_hi, o, 64));
+    }
+    lim_lo = __builtin_amdgcn_readfirstlane(lim_lo);
+    start_hi = __builtin_amdgcn_readfirstlane(start_hi);
+
+    // ---- query operands (zeros for absent columns)
+    Op qB[KS];
+    Op qbias = Op{};  // affine: the query's sum over each group as fp16 hi + lo at 2 g, 2 g + 1 (lanes of half 0)
+    {
+      const bool ok = tok >= 0;
+      const QT* qp = reinterpret_cast<const QT*>(a.q) +
+                     ((size_t)(ok ? q0 + tok : 0) * a.Hq + (size_t)kvh * HG + (ok ? head : 0)) * D + 8 * half;
+      float gsum[G] = {};
+#pragma unroll
+      for (int w2 = 0; w2 < KS; ++w2) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * w2);
+        const Op v = __builtin_bit_cast(Op, ok ? x : u32x4{0u, 0u, 0u, 0u});
+        if constexpr (AFF) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            qB[w2][i] = v[slot_perm<C::kBits>(i)];  // the unpacked codes' order
+            gsum[w2 * G / KS] += (float)v[i];
+          }
+        } else {
+          qB[w2] = v;
+        }
+      }
+      if constexpr (AFF) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float x = gsum[g] + __shfl_xor(gsum[g], 32, 64);
+          const h16 hi = (h16)x;
+          if (half == 0) {
+            qbias[2 * g] = hi;
+            qbias[2 * g + 1] = (h16)(x - (float)hi);
+          }
+        }
+      }
+    }
+
+    float m_run = -INFINITY, l_part = 0.f;
+    f32x16 acc[DT];
+    float pb[G] = {};  // affine: sum p * v_bias
+    int vexp = 0;      // FP8, affine: acc holds the sum / 2^vexp
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+
+    if constexpr (AFF) {  // the bias operand's unused halves stay zero
+      for (int i = tid; i < 2 * NT; i += 256)
+        *reinterpret_cast<u32x4*>(lds + oBuf + (i / NT) * BUF + oSc + 12 * G * NT + 16 * (i % NT)) = u32x4{0u, 0u, 0u, 0u};
+      __syncthreads();
+    }
+    if (st_lo < st_hi) store_block(st_lo, 0);
+    __syncthreads();
+
+    for (int st = st_lo; st < st_hi; ++st) {
+      const int buf = (st - st_lo) & 1;
+      const uint64_t okm = okn;
+      if (st + 1 < st_hi) {
+        load_block(st + 1, blk1);
+        blk1 = page_id(min(st + 2, st_hi - 1));
+      }
+      const unsigned char* img = lds + oBuf + buf * BUF;
+      if (busy) {
+        const float* ksf = reinterpret_cast<const float*>(img + oSc);
+        if constexpr (AFF || FP8) {
+          const int ex = __builtin_amdgcn_readfirstlane(*reinterpret_cast<const int*>(img + oSc + P::SCB));
+          if (ex != vexp) {
+            const float f = __uint_as_float((uint32_t)(127 + min(max(vexp - ex, -126), 127)) << 23);
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+            vexp = ex;
+          }
+        }
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4* lds4;
+        const int ki = oBuf + buf * BUF + kad, vi = oBuf + buf * BUF + vad;
+        auto read_k = [&](const int kt, const int w2) {
+          return *reinterpret_cast<const Op*>(lds + (ki ^ (w2 << 5)) + kt * 64 * D);
+        };
+        auto read_v = [&](const int kt, const int j, const int d) {
+          if constexpr (AFF) {
+            return *reinterpret_cast<const Op*>(lds + (vi ^ ((4 * kt + 2 * j) << 4)) + d * 64 * NT);
+          } else {
+            const unsigned char* p = lds + (vi ^ (d << 6)) + (32 * kt + 16 * j) * (D * 2);
+            const u32x2 v0 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p)));
+            const u32x2 v1 = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 8 * (D * 2))));
+            return __builtin_bit_cast(Op, u32x4{v0[0], v0[1], v1[0], v1[1]});
+          }
+        };
+        // Operands are read ahead of the products that take them, held in that order by the barriers (the compiler
+        // put each read right before its use: a wait of the whole LDS latency per product)
+        constexpr int KA = KS < 4 ? KS : 4;  // K operands read ahead
+        Op ka[KA];
+#pragma unroll
+        for (int i = 0; i < KA; ++i) ka[i] = read_k(KT - 1, i);
+#pragma unroll
+        for (int kk = 0; kk < KT; ++kk) {
+          const int kt = KT - 1 - kk;  // backwards, as the cursors go; 32 keys at a time: their scores alone are in registers
+          const int k0 = (kw * KT + kt) * 32;
+          __builtin_amdgcn_sched_barrier(0);
+          // ---- S^T: element i is key 8 (i / 4) + 4 half + i % 4 of the 32
+          f32x16 sc;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+          if constexpr (AFF) {
+            const h16* kbe = reinterpret_cast<const h16*>(ksf + 3 * G * NT);
+            sc = mfma32(*reinterpret_cast<const Op*>(kbe + 8 * (k0 + c32)), qbias, sc);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+              f32x16 c;
+#pragma unroll
+              for (int i = 0; i < 16; ++i) c[i] = 0.f;
+#pragma unroll
+              for (int w2 = g * KS / G; w2 < (g + 1) * KS / G; ++w2)
+                c = mfma32(w2 < KA ? ka[w2 < KA ? w2 : 0] : read_k(kt, w2), qB[w2], c);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const f32x4 ks4 = *reinterpret_cast<const f32x4*>(ksf + g * NT + k0 + 8 * j + 4 * half);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[4 * j + r] = fmaf(c[4 * j + r], ks4[r], sc[4 * j + r]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int w2 = 0; w2 < KS; ++w2)
+              sc = mfma32(w2 < KA ? ka[w2 < KA ? w2 : 0] : read_k(kt, w2), qB[w2], sc);
+            if constexpr (FP8) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const f32x4 ks4 = *reinterpret_cast<const f32x4*>(ksf + k0 + 8 * j + 4 * half);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sc[4 * j + r] *= ks4[r];
+              }
+            }
+          }
+
+          // ---- mask, where some key is not visible to every column of the wave
+          const int kp = pos_of_block(st) + k0;
+          const uint32_t okw = (uint32_t)(okm >> k0);
+          const bool drafted = tree && kp + 32 > past;
+          const bool full = !drafted && kp + 31 <= lim_lo && (kp >= start_hi || kp + 32 <= mask.sinks) &&
+                            okw == 0xFFFFFFFFu;
+          if (!full) {
+            // bit k: the column sees key kp + k
+            uint32_t see = below(limit + 1 - kp) & (~below(start - kp) | below(mask.sinks - kp));
+            if (drafted) {
+              while (cur >= 0 && past + cur >= kp) {
+                const int b = past + cur - kp;
+                if (b < 32 && (mask.window <= 0 || back < mask.window || place - back < mask.sinks)) see |= 1u << b;
+                cur = up(cur);
+                ++back;
+              }
+            }
+            see = (see & okw) >> (4 * half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] = (see >> (8 * (i / 4) + i % 4)) & 1u ? sc[i] : -INFINITY;
+          }
+
+          // ---- online softmax: the lane's own scores of its column
+          float top = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, sc[i]), sc[i + 1]);
+          if (__any(top * sl2 > m_run + kLazyMax)) {
+            const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32, 64)) * sl2);
+            const bool rise = m_new > m_run + kLazyMax;  // also the first finite maximum
+            const float al = rise ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+            l_part *= al;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= al;
+            if constexpr (AFF) {
+#pragma unroll
+              for (int g = 0; g < G; ++g) pb[g] *= al;
+            }
+            if (rise) m_run = m_new;
+          }
+          constexpr int DG = DT / G;  // dim tiles of a quantization group
+          Op va[DT];
+          if constexpr (!AFF) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d) va[d] = read_v(kt, 0, d);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          // p <= 2^(kLazyMax + 6), times a value scale below 2: inside fp16, and small p stay clear of its sub-normals
+          const float m_sub = fmaxf(m_run, -3.0e38f) - 6.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], sl2, -m_sub));
+            l_part += sc[i];
+          }
+          // ---- O^T += V^T P^T, 16 keys at a time
+          if constexpr (AFF) {
+            const float *vsf = ksf + G * NT, *vbf = vsf + G * NT;
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int g = 0; g < G; ++g) {
+#pragma unroll
+                for (int d = 0; d < DG; ++d) va[d] = read_v(kt, j, g * DG + d);
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const f32x4 vs4 = *reinterpret_cast<const f32x4*>(vsf + g * NT + k0 + 16 * j + 8 * e + 4 * half);
+                  const f32x4 vb4 = *reinterpret_cast<const f32x4*>(vbf + g * NT + k0 + 16 * j + 8 * e + 4 * half);
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) {
+                    const float p = sc[8 * j + 4 * e + r];
+                    x[4 * e + r] = p * vs4[r];
+                    pb[g] = fmaf(p, vb4[r], pb[g]);
+                  }
+                }
+                Op pB[2];
+                split_p2(x, pB);
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                  for (int d = 0; d < DG; ++d) acc[g * DG + d] = mfma32(va[d], pB[k], acc[g * DG + d]);
+                __builtin_amdgcn_sched_barrier(0);  // (the scales' reads stay with their group)
+              }
+            if (kk + 1 < KT) {
+#pragma unroll
+              for (int i = 0; i < KA; ++i) ka[i] = read_k(kt - 1, i);
+            }
+          } else {
+            Op pB[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = sc[8 * j + e];
+              if constexpr (FP8) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const f32x4 vs4 = *reinterpret_cast<const f32x4*>(ksf + NT + k0 + 16 * j + 8 * e + 4 * half);
+#pragma unroll
+                  for (int r = 0; r < 4; ++r) x[4 * e + r] *= vs4[r];
+                }
+              }
+              split_p2(x, pB[j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            Op vb[DT];
+#pragma unroll
+            for (int d = 0; d < DT; ++d) vb[d] = read_v(kt, 1, d);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int d = 0; d < DT; ++d) acc[d] = mfma32(va[d], pB[0][k], acc[d]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (kk + 1 < KT) {
+#pragma unroll
+              for (int i = 0; i < KA; ++i) ka[i] = read_k(kt - 1, i);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int d = 0; d < DT; ++d) acc[d] = mfma32(vb[d], pB[1][k], acc[d]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (st + 1 < st_hi) store_block(st + 1, buf ^ 1);
+      __syncthreads();
+    }
+
+    if constexpr (AFF) {  // codes entered as code * 2^-kCodeExp; the bias term joins its group's dims
+      const float f = __uint_as_float((uint32_t)(127 + vexp + C::kCodeExp) << 23);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float bias = pb[g] + __shfl_xor(pb[g], 32, 64);
+#pragma unroll
+        for (int d = g * DT / G; d < (g + 1) * DT / G; ++d) acc[d] = acc[d] * f + bias;
+      }
+    }
+    if constexpr (FP8) {  // the codes entered as value * 2^-8
+      const float f = __uint_as_float((uint32_t)(127 + vexp + 8) << 23);
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[d] *= f;
+    }
+    float l = l_part + __shfl_xor(l_part, 32, 64);
+
+    // ---- KW = 2: the second key wave's state joins the first's
+    if constexpr (KW > 1) {
+      f32x4* meet = reinterpret_cast<f32x4*>(lds + oBuf) + (size_t)cw * (4 * DT + 1) * 64 + lane;
+      if (kw == 1) {
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            meet[(4 * d + j) * 64] = f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+        meet[4 * DT * 64] = f32x4{m_run, l, 0.f, 0.f};
+      }
+      __syncthreads();
+      if (kw == 0) {
+        const f32x4 o = meet[4 * DT * 64];
+        const float M = fmaxf(m_run, o[0]);
+        // (a wave without a live key has m = -inf and zeros, one of NaN scores only a sum that is NaN)
+        const float f0 = m_run == -INFINITY ? (l == 0.f ? 0.f : l) : __builtin_amdgcn_exp2f(m_run - M);
+        const float f1 = o[0] == -INFINITY ? (o[1] == 0.f ? 0.f : o[1]) : __builtin_amdgcn_exp2f(o[0] - M);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 y = meet[(4 * d + j) * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[d][4 * j + r] = acc[d][4 * j + r] * f0 + y[r] * f1;
+          }
+        l = l * f0 + o[1] * f1;
+        m_run = M;
+      }
+    }
+
+    const bool whole = b0 == 0 && b1 == nblk;
+    if (nwg > 0 && b0 == 0 && tid == 0) {
+      // who has the tile's last block, counting this range's as the first
+      const int g0 = (int)((long long)(w + 1) * all / nwg) - todo;  // the tile's first block in the launch
+      const int wl = whole ? w : (int)(((long long)(g0 + nblk) * nwg - 1) / all);
+      A.desc[1 + (size_t)kvh * A.tiles + t] = int4{sq.s, tile, whole ? 1 : wl - w + 1, 2 * w + (first_seg ? 0 : 1)};
+    }
+    if (kw == 0) {
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            bad |= masked_write<C, D>(a, sq, kvh, tok, head,
+                                      f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, l,
+                                      inv, 32 * d + 8 * j + 4 * half);
+        uint64_t again = __ballot(bad);
+        again = (again | (again >> 32)) & 0xFFFFFFFFull;
+        if (again) {
+          __builtin_amdgcn_s_waitcnt(0);  // (the rows' first results are out before their second)
+          for (; again; again &= again - 1) {
+            const int c = __builtin_ctzll(again);
+            attend_masked<C, D>(a, mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c),
+                                lane);
+          }
+        }
+      } else {
+        f32x4* st = reinterpret_cast<f32x4*>(A.part + (size_t)(2 * w + (first_seg ? 0 : 1)) * kWidePart<D, KW>) +
+                    (size_t)cw * (D / 8 + 1) * 64 + lane;
+        if (tok >= 0) {
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              st[(4 * d + j) * 64] = f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+        }
+        st[(D / 8) * 64] = f32x4{m_run, l, 0.f, 0.f};
+      }
+    }
+    if (nwg == 0) return;
+    todo -= b1 - b0;
+    if (todo <= 0) return;
+    first_seg = false;
+    b0 = 0;
+    if (++t == ntiles) {
+      t = 0;
+      ++kvh;
+      sidx = 0;
+    }
+  }
+}
+
+// Joins the parts of cut tiles, in part order.  Grid (tiles * Hkv, column waves, D / 32): a workgroup has 32 columns and
+// 32 dims of one tile, a wave 8 of them, 8 parts in flight.
+template <class C, int D, int KW>
+__global__ __launch_bounds__(256) void masked_merge(MaskedArgs A) {
+  const DecodeArgs& a = A.d;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), cw = blockIdx.y;
+  const int kvh = blockIdx.x / A.tiles, t = blockIdx.x % A.tiles;
+  if (t >= A.desc[0].x) return;
+  const int4 de = A.desc[1 + blockIdx.x];
+  const int np = de.z;
+  if (np <= 1) return;
+  const int c32 = lane & 31, half = lane >> 5, vec = 4 * blockIdx.z + wv;
+  const f32x4* base = reinterpret_cast<const f32x4*>(A.part) + (size_t)cw * (D / 8 + 1) * 64 + lane;
+  // the first part's slot, then the first slots of the workgroups that follow
+  const int slot0 = de.w, next0 = (de.w | 1) + 1;
+  auto slot = [&](const int q) { return (size_t)(q == 0 ? slot0 : next0 + 2 * (q - 1)) * (kWidePart<D, KW> / 4); };
+  constexpr int U = 8;
+  const MaskedSeq sq = masked_seq(A, de.x);
+  float m = -INFINITY, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int q0 = 0; q0 < np; q0 += U) {
+    f32x4 x[U];
+    f32x2 ml[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {  // (past the last part: that one again, of no weight)
+      const f32x4* st = base + slot(min(q0 + k, np - 1));
+      ml[k] = *reinterpret_cast<const f32x2*>(st + (D / 8) * 64);
+      x[k] = st[vec * 64];  // (a column that is none holds anything: its lanes write nothing)
+    }
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < U; ++k) top = fmaxf(top, ml[k][0]);
+    // (a part without a live key has m = -inf and zeros, one of NaN scores only a sum that is NaN)
+    auto weight = [&](const float m1, const float l1) {
+      return m1 == -INFINITY ? (l1 == 0.f ? 0.f : l1) : __builtin_amdgcn_exp2f(m1 - top);
+    };
+    const float f0 = weight(m, l);
+    l *= f0;
+    o *= f0;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (q0 + k < np) {
+        const float f = weight(ml[k][0], ml[k][1]);
+        l = fmaf(ml[k][1], f, l);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = fmaf(x[k][r], f, o[r]);
+      }
+    }
+    m = top;
+  }
+  int tok, head;
+  masked_column(A, sq, de.y, cw * 32 + c32, a.Hq / a.Hkv, tok, head);
+  const bool bad = masked_write<C, D>(a, sq, kvh, tok, head, o, l, l > 0.f ? 1.f / l : 0.f,
+                                      32 * (vec / 4) + 8 * (vec % 4) + 4 * half);
+  // rows that are not finite here: these 32 dims again in fp32
+  __shared__ unsigned int again[4];
+  const uint64_t b = __ballot(bad);
+  if (lane == 0) again[wv] = (unsigned int)(b | (b >> 32));
+  __builtin_amdgcn_s_waitcnt(0);  // (the first results are out before the second)
+  __syncthreads();
+  unsigned int all = __builtin_amdgcn_readfirstlane(again[0] | again[1] | again[2] | again[3]);
+  for (; all; all &= all - 1) {
+    const int c = __builtin_ctz(all);
+    if ((c & 3) == wv)
+      attend_masked<C, D>(a, A.mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c),
+                          lane, 32 * blockIdx.z, 32 * blockIdx.z + 32);
+  }
+}
+
+}  // namespace emx
