@@ -7,6 +7,7 @@ missing every entry point raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -121,6 +122,16 @@ def stream_ptr(device) -> int:
 
 _raw_stream = None
 _torch = None
+_same_device = contextlib.nullcontext()
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one (kernels launch on the current device)"""
+    import torch
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _same_device
+    return torch.cuda.device(device)
 
 
 def load() -> ctypes.CDLL:

@@ -105,7 +105,7 @@ class PageCacheConfig:
 class PageCache:
     """Per-layer :class:`PageCacheView` container (``cache.py:1370-1445``)."""
 
-    __slots__ = ("config", "views")
+    __slots__ = ("_commit_plan", "config", "views")
 
     def __init__(self, views: list[PageCacheView], config: PageCacheConfig | None = None) -> None:
         self.views = views
@@ -159,9 +159,14 @@ class PageCache:
     def commit_tree(self, path, accepted, query_start_loc, *, slot_ids=None) -> None:
         """Keep the accepted path of every drafted tree in every layer
         (:func:`~easymlx_amd.caching.tree.commit_tree`): up to 32 layers of one shape move in one launch."""
-        from .tree import commit_tree
+        from .tree import CommitPlan, commit_tree
 
-        commit_tree(self.views, path, accepted, query_start_loc, slot_ids=slot_ids)
+        if not self.views:
+            return
+        plan = getattr(self, "_commit_plan", None)
+        if plan is None or not plan.fits(self.views):
+            plan = self._commit_plan = CommitPlan(self.views)
+        commit_tree(self.views, path, accepted, query_start_loc, slot_ids=slot_ids, plan=plan)
 
     def zero_pages(self, page_ids) -> None:
         """The runner's ``_zero_pages`` over every layer (``model_runner.py:1058-1094``)."""

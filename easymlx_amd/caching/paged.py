@@ -250,7 +250,8 @@ class PageCacheView:
         parents = getattr(cache_metadata, "tree_parents", None)
         if parents is None:
             return None
-        parents = torch.as_tensor(parents)
+        if not isinstance(parents, torch.Tensor):
+            parents = torch.as_tensor(parents)
         if parents.ndim != 1 or parents.is_floating_point() or parents.is_complex():
             raise ValueError("tree_parents must be rank-1 integers: [total_tokens]")
         if int(parents.shape[0]) != sum(max(0, n) for n in qlens):

@@ -10,6 +10,7 @@ moves whole pages.
 from __future__ import annotations
 
 import ctypes
+import operator
 import typing as tp
 
 import torch
@@ -19,19 +20,88 @@ from .. import _native
 
 def _shape_of(view) -> tuple:
     """What the layers of one launch have alike."""
-    return (type(view).page_arrays, view.num_seqs, view.blocks_per_seq, view.num_blocks, view.block_size,
-            view.num_kv_heads, view.head_dim, view.key_cache.dtype, getattr(view, "bits", None),
-            getattr(view, "group_size", None), view.key_cache.device)
+    return (type(view).page_arrays, view.block_tables.shape, view.key_cache.shape, view.value_cache.shape,
+            view.block_size, view.num_kv_heads, view.head_dim, view.key_cache.dtype, getattr(view, "bits", None),
+            getattr(view, "group_size", None))
+
+
+def _pointers(tensors):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+class CommitPlan:
+    """The arrays of several layers, checked and laid out for the launches of :func:`commit_tree`.
+
+    A :class:`~easymlx_amd.caching.pagecache.PageCache` keeps one for its views: checking the arrays of 32 layers and
+    listing their addresses takes longer than moving the rows.  :meth:`fits` tells whether the views still hold
+    those very tensors at those addresses.
+    """
+
+    def __init__(self, views: tp.Sequence[tp.Any]):
+        self.views = list(views)
+        dev = self.device = self.views[0].key_cache.device
+        self.num_seqs = min(v.num_seqs for v in self.views)
+        for v in self.views:
+            if v.block_tables.dtype != torch.int32 or v.kv_lens.dtype != torch.int32:
+                raise ValueError("block_tables and kv_lens must be int32")
+            arrays = [*v.page_arrays(), v.block_tables, v.kv_lens]
+            if any(not t.is_contiguous() for t in arrays):
+                raise ValueError("commit_tree changes caches in place: they, tables and lengths must be contiguous")
+            if any(t.device != dev for t in arrays):
+                raise ValueError("the layers' caches, tables and lengths must be on one device")
+        self.tensors = self._tensors(self.views)
+        self.addresses = [t.data_ptr() for t in self.tensors]
+        # runs of layers of one shape; a run that shared its lengths with another would see them change between the two
+        runs: list[list] = []
+        for v in self.views:
+            if runs and _shape_of(runs[-1][0]) == _shape_of(v):
+                runs[-1].append(v)
+            else:
+                runs.append([v])
+        seen: dict[int, int] = {}
+        for i, run in enumerate(runs):
+            for v in run:
+                if seen.setdefault(v.kv_lens.data_ptr(), i) != i:
+                    raise ValueError("layers of different shapes cannot share kv_lens")
+        self.runs = [self._run(r) for r in runs]
+
+    @staticmethod
+    def _tensors(views) -> list[torch.Tensor]:
+        return [t for v in views for t in (*v.page_arrays(), v.block_tables, v.kv_lens)]
+
+    @staticmethod
+    def _run(views) -> tuple:
+        """(affine, arguments before the trees, the sequences' arguments) of a run's C call."""
+        v = views[0]
+        seqs = (_pointers([x.block_tables for x in views]), v.num_seqs, v.blocks_per_seq,
+                _pointers([x.kv_lens for x in views]))
+        if v.is_affine:
+            return True, (len(views), _pointers([t for x in views for t in x.page_arrays()]), v.num_kv_heads,
+                          v.head_dim, v.bits, v.group_size, v.block_size, v.num_blocks), seqs
+        row = v.num_kv_heads * v.head_dim * v.key_cache.element_size()
+        return False, (len(views), _pointers([x.key_cache for x in views]), _pointers([x.value_cache for x in views]),
+                       row, v.block_size, v.num_blocks), seqs
+
+    def fits(self, views) -> bool:
+        if len(views) != len(self.views) or not all(map(operator.is_, views, self.views)):
+            return False
+        now = self._tensors(views)
+        return (len(now) == len(self.tensors) and all(map(operator.is_, now, self.tensors))
+                and [t.data_ptr() for t in now] == self.addresses)
 
 
 def _index(name: str, x, device) -> torch.Tensor:
-    x = torch.as_tensor(x)
+    if not isinstance(x, torch.Tensor):
+        x = torch.as_tensor(x)
     if x.ndim != 1 or x.is_floating_point() or x.is_complex():
         raise ValueError(f"{name} must be rank-1 integers")
+    if x.dtype == torch.int32 and x.device == device and x.is_contiguous():
+        return x
     return x.to(device=device, dtype=torch.int32).contiguous()
 
 
-def commit_tree(views: tp.Sequence[tp.Any], path, accepted, query_start_loc, *, slot_ids=None) -> None:
+def commit_tree(views: tp.Sequence[tp.Any], path, accepted, query_start_loc, *, slot_ids=None,
+                plan: CommitPlan | None = None) -> None:
     """Keep the accepted path of every drafted tree in the caches of ``views`` (one per layer).
 
     Tree ``i`` is the last ``q = query_start_loc[i + 1] - query_start_loc[i]`` tokens of sequence ``slot_ids[i]``
@@ -40,19 +110,21 @@ def commit_tree(views: tp.Sequence[tp.Any], path, accepted, query_start_loc, *, 
     layer; layers that share their ``kv_lens`` tensor see it change once.  ``path`` ascends inside a tree, as
     :func:`~easymlx_amd.operations.tree_attention.tree_accept` returns it.  Affine pages move codes, scales and biases
     as they are, FP8 pages codes: a tree's rows are written with one scale.  A sequence may appear once.
-    Everything stays on the device: a step with this call can be captured in a graph.
+    Everything stays on the device: a step with this call can be captured in a graph.  ``plan``: the views'
+    :class:`CommitPlan`, made for the call without it.
     """
-    views = list(views)
     if not views:
         return
-    dev = views[0].key_cache.device
+    if plan is None:
+        plan = CommitPlan(views)
+    dev = plan.device
     path, accepted = _index("path", path, dev), _index("accepted", accepted, dev)
     qsl = _index("query_start_loc", query_start_loc, dev)
     n = int(accepted.shape[0])
     if int(qsl.shape[0]) != n + 1:
         raise ValueError("query_start_loc must have one entry more than accepted")
     if slot_ids is None:
-        if any(n > v.num_seqs for v in views):
+        if n > plan.num_seqs:
             raise ValueError("more trees than sequences")
     else:
         if not isinstance(slot_ids, torch.Tensor):
@@ -63,55 +135,22 @@ def commit_tree(views: tp.Sequence[tp.Any], path, accepted, query_start_loc, *, 
             raise ValueError("slot_ids must be rank-1")
         if len(slot_ids) != n:
             raise ValueError("slot_ids must hold one sequence per tree")
-    for v in views:
-        if v.block_tables.dtype != torch.int32 or v.kv_lens.dtype != torch.int32:
-            raise ValueError("block_tables and kv_lens must be int32")
-        if not v.kv_lens.is_contiguous() or any(not t.is_contiguous() for t in v.page_arrays()):
-            raise ValueError("commit_tree changes caches and kv_lens in place: they must be contiguous")
-        if v.key_cache.device != dev or v.block_tables.device != dev or v.kv_lens.device != dev:
-            raise ValueError("the layers' caches, tables and lengths must be on one device")
     if dev.type != "cuda":
         raise RuntimeError("commit_tree runs on the GPU only; the cache is on " + str(dev))
-    if n == 0 or int(path.shape[0]) == 0:
+    total = int(path.shape[0])
+    if n == 0 or total == 0:
         return
+    slots = None
     if slot_ids is not None:
-        slot_ids = (views[0]._slot_ids_device(slot_ids) if isinstance(slot_ids, tuple)
-                    else slot_ids.to(device=dev, dtype=torch.int32).contiguous())
-    # runs of layers of one shape; a run that shares its lengths with another would see them change between the two
-    runs: list[list] = []
-    for v in views:
-        if runs and _shape_of(runs[-1][0]) == _shape_of(v):
-            runs[-1].append(v)
-        else:
-            runs.append([v])
-    if len(runs) > 1:
-        seen: dict[int, int] = {}
-        for i, run in enumerate(runs):
-            for v in run:
-                if seen.setdefault(v.kv_lens.data_ptr(), i) != i:
-                    raise ValueError("layers of different shapes cannot share kv_lens")
-    with torch.cuda.device(dev):
-        stream = _native.stream_ptr(dev)
-        for run in runs:
-            _commit(run, path, accepted, qsl, slot_ids, n, stream)
+        slot_ids = (plan.views[0]._slot_ids_device(slot_ids) if isinstance(slot_ids, tuple)
+                    else _index("slot_ids", slot_ids, dev))
+        slots = slot_ids.data_ptr()
+    lib = _native.load()
+    with _native.on_device(dev):
+        trees = (slots, n, path.data_ptr(), accepted.data_ptr(), qsl.data_ptr(), total, _native.stream_ptr(dev))
+        for affine, arrays, seqs in plan.runs:
+            call = lib.emx_tree_commit_affine if affine else lib.emx_tree_commit_rows
+            _native.check(call(*arrays, *seqs, *trees))
 
 
-def _commit(views, path, accepted, qsl, slot_ids, n, stream) -> None:
-    lib, v0, m = _native.load(), views[0], len(views)
-    tables = [v.block_tables.contiguous() for v in views]
-    pointers = lambda ts: (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts])  # noqa: E731
-    tree = (pointers(tables), v0.num_seqs, v0.blocks_per_seq, pointers([v.kv_lens for v in views]),
-            None if slot_ids is None else slot_ids.data_ptr(), n, path.data_ptr(), accepted.data_ptr(), qsl.data_ptr(),
-            int(path.shape[0]), stream)
-    if v0.is_affine:
-        rc = lib.emx_tree_commit_affine(m, pointers([t for v in views for t in v.page_arrays()]), v0.num_kv_heads,
-                                        v0.head_dim, v0.bits, v0.group_size, v0.block_size, v0.num_blocks, *tree)
-    else:
-        rc = lib.emx_tree_commit_rows(m, pointers([v.key_cache for v in views]),
-                                      pointers([v.value_cache for v in views]),
-                                      v0.num_kv_heads * v0.head_dim * v0.key_cache.element_size(), v0.block_size,
-                                      v0.num_blocks, *tree)
-    _native.check(rc)
-
-
-__all__ = ("commit_tree",)
+__all__ = ("CommitPlan", "commit_tree")

@@ -85,7 +85,10 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, tree_parents, query
         raise ValueError("tokens and targets must be rank-1 of one length: [total_tokens]")
     if tokens.dtype not in (torch.int32, torch.int64) or targets.dtype != tokens.dtype:
         raise ValueError("tokens and targets must be int32 or int64, both the same")
-    tree_parents, query_start_loc = torch.as_tensor(tree_parents), torch.as_tensor(query_start_loc)
+    if not isinstance(tree_parents, torch.Tensor):
+        tree_parents = torch.as_tensor(tree_parents)
+    if not isinstance(query_start_loc, torch.Tensor):
+        query_start_loc = torch.as_tensor(query_start_loc)
     if tree_parents.shape != tokens.shape or tree_parents.is_floating_point():
         raise ValueError("tree_parents must be rank-1 integers: [total_tokens]")
     if query_start_loc.ndim != 1 or query_start_loc.shape[0] < 1:
@@ -101,7 +104,7 @@ def tree_accept(tokens: torch.Tensor, targets: torch.Tensor, tree_parents, query
     path = torch.empty((total,), dtype=torch.int32, device=dev)
     accepted = torch.empty((n,), dtype=torch.int32, device=dev)
     following = torch.empty((n,), dtype=tokens.dtype, device=dev)
-    with torch.cuda.device(dev):
+    with _native.on_device(dev):
         _native.check(_native.load().emx_tree_accept(
             tokens.data_ptr(), targets.data_ptr(), tokens.element_size(), parents.data_ptr(), qsl.data_ptr(), n, total,
             path.data_ptr(), accepted.data_ptr(), following.data_ptr(), _native.stream_ptr(dev)))

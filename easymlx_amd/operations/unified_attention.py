@@ -178,8 +178,11 @@ def _masked_attention(queries, key_cache, value_cache, block_tables, kv_lens, qu
     """The call with sinks or a drafted tree: ``emx_masked_attention_*`` on checked, device-resident arguments."""
     dev = queries.device
     total, hq, d = (int(x) for x in queries.shape)
-    caches = [t for t in (key_cache, value_cache, k_scale, v_scale, k_scales, k_biases, v_scales, v_biases)
-              if t is not None]
+    caches = [key_cache, value_cache]
+    if affine:
+        caches += [k_scales, k_biases, v_scales, v_biases]
+    elif k_scale is not None and v_scale is not None:
+        caches += [k_scale, v_scale]
     if any(t.device != dev for t in caches):
         raise ValueError(f"the cache must be on the queries' device {dev}")
     if out.shape != queries.shape or out.dtype != queries.dtype or out.device != dev or not out.is_contiguous():
@@ -208,7 +211,7 @@ def _masked_attention(queries, key_cache, value_cache, block_tables, kv_lens, qu
             if k_scale.numel() != nb or v_scale.numel() != nb:
                 raise ValueError("k_scale/v_scale must hold one scale per block: [num_blocks]")
     lib = _native.load()
-    with torch.cuda.device(dev):
+    with _native.on_device(dev):
         stream = _native.stream_ptr(dev)
         if workspace is None:
             workspace = _workspace(dev, stream, _masked_bytes(total, S, hq, hkv, d), own=True)
@@ -312,7 +315,8 @@ def paged_attention(
     if sink_tokens < 0:
         raise ValueError(f"sink_tokens must be >= 0, got {sink_tokens}")
     if tree_parents is not None:
-        tree_parents = torch.as_tensor(tree_parents)
+        if not isinstance(tree_parents, torch.Tensor):
+            tree_parents = torch.as_tensor(tree_parents)
         if tree_parents.ndim != 1 or int(tree_parents.shape[0]) != total:
             raise ValueError("tree_parents must be rank-1: [total_tokens]")
         if total and (tree_parents.is_floating_point() or tree_parents.is_complex()):

@@ -149,6 +149,27 @@ def test_commit_slots_shared_lengths_many_layers(cuda):
     np.testing.assert_array_equal(views[0].kv_lens.cpu().numpy(), exp[0][0][1])
 
 
+def test_commit_follows_replaced_tensors(cuda):
+    """A cache whose tensors, or views, are replaced between two commits: the new ones change."""
+    path, qsl = torch.tensor([0, 2, -1], dtype=torch.int32, device=cuda), [0, 3]
+    count = torch.tensor([2], dtype=torch.int32, device=cuda)
+    cache = PageCache([view_of("f16", cuda, seed=s) for s in (1, 2)])
+    for change in (lambda: None, lambda: setattr(cache[0], "key_cache", cache[0].key_cache.clone()),
+                   lambda: setattr(cache[1], "kv_lens", torch.zeros_like(cache[1].kv_lens)),
+                   lambda: cache.__setitem__(0, view_of("q8", cuda, seed=4)), lambda: cache.views.pop()):
+        change()
+        exp = []
+        for v in cache:
+            v.kv_lens.copy_(torch.tensor([40, 0, 0, 0, 0], dtype=torch.int32))
+            exp.append([masked.tree_commit(x, v.block_tables.cpu().numpy(), [40, 0, 0, 0, 0], [0, 2, -1], [2], qsl)
+                        for x in rows_of(v)])
+        cache.commit_tree(path, count, qsl)
+        for v, r in zip(cache, exp):
+            for got, (rows, lens) in zip(rows_of(v), r):
+                np.testing.assert_array_equal(got, rows)
+                np.testing.assert_array_equal(v.kv_lens.cpu().numpy(), lens)
+
+
 def test_commit_bad_pages_and_paths(cuda):
     """Pages outside the pool, a tree that starts before its sequence, entries that do not ascend: left alone."""
     v = view_of("q8", cuda, page=8)
