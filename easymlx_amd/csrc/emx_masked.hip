@@ -14,21 +14,30 @@ namespace emx {
 // Workgroups that the chip holds at once, two to a compute unit; a call of fewer tiles is cut.
 constexpr int kMaskedWGs = 512;
 
-MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, bool cut) {
+constexpr int kMaskedHeads = 128;  // query heads of a kv head: a tile's columns
+
+MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, KvKind kind, bool cut) {
   MaskedShape m{};
   const int hg = Hq / Hkv;
-  if (hg <= 0 || T <= 0 || S <= 0) return m;
-  // sequences of up to 64 columns on average (small trees): two waves to a column, half of the keys each
-  m.kw = D <= 128 && hg <= 64 && (long)T * hg <= 64L * S ? 2 : 1;
-  if (hg > 128 / m.kw) return m;
-  m.tokb = 128 / m.kw / hg;
+  if (hg <= 0 || hg > kMaskedHeads || T <= 0 || S <= 0) return m;
+  const bool plain = kind == KvKind::f16 || kind == KvKind::bf16;
+  const long cols = (long)T * hg;  // query columns of all sequences, per kv head
+  // Sequences of up to 64 columns on average (small trees): two waves to a column, half of the keys each.  Else, where tiles
+  // are few, 256 columns: each block of the cache is read half as often (12 trees of 48 to 64 nodes, 64 / 8 heads, up to
+  // 32768 keys: 745 us against 896; 8 of 31 to 60, 32 / 8 heads: 73 against 80); where they are many, 128: two workgroups to
+  // a compute unit, one begins a tile while the other multiplies (four prompts, window 1024: 252 us against 262).
+  m.cw = D <= 128 && hg <= 64 && cols <= 64L * S ? 2 : 4;
+  if (plain && D == 128 && m.cw == 4 && cols > 128L * S && cols * Hkv < 256L * kMaskedWGs) m.cw = 8;
+  m.tokb = 32 * m.cw / hg;
   // a sequence of q query tokens has at most q / tokb + 1 tiles
   const long least = ((long)T + m.tokb - 1) / m.tokb;
   m.tiles = least + std::min(S, T);
-  if (cut && least * Hkv < 2 * kMaskedWGs) {
-    m.wgs = D == 256 ? kMaskedWGs / 2 : kMaskedWGs;  // (its registers: one workgroup to a compute unit)
-    m.desc_bytes = 16 * (size_t)(1 + m.tiles * Hkv);
-    m.part_bytes = 2 * (size_t)m.wgs * (4 / m.kw) * (D / 8 + 1) * 1024;
+  // (of 512 threads: one to a compute unit)
+  const int wgs = D == 256 || m.cw == 8 || (D == 128 && m.cw == 4 && kind == KvKind::affine) ? kMaskedWGs / 2 : kMaskedWGs;
+  if (cut && least * Hkv < 2 * wgs) {
+    m.wgs = wgs;
+    m.desc_bytes = 16 * (size_t)(1 + std::min<long>(m.tiles * Hkv, wgs));
+    m.part_bytes = 2 * (size_t)m.wgs * m.cw * (D / 8 + 1) * 1024;
   }
   return m;
 }
@@ -101,7 +110,7 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
     return false;
   const size_t base = workspace_base();
   // rows of one token: the split-K decode (a tile of the kernel below would hold a group's heads alone)
-  const size_t rows = g.decode && c.mask.sinks > 0 && !c.mask.parents
+  const size_t rows = g.decode && c.mask.sinks > 0 && !c.mask.parents && g.Hq / g.Hkv <= kMaskedHeads
                           ? decode_mfma_partial_bytes(g.S, g.Hq, g.Hkv, g.D) : 0;
   if (rows && c.ws && c.ws_bytes >= base + rows) {
     launch_masked_rows(m, c.mask.sinks, static_cast<int*>(c.ws),
@@ -109,12 +118,12 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
     *rc = entry_check_launch("decode_mfma (sinks)");
     return true;
   }
-  MaskedShape shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, true);
+  MaskedShape shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, m.kind, true);
   if (shape.tokb == 0) return false;
   // (the blocks of a cut launch are counted in 31 bits)
   if (shape.wgs && (!c.ws || c.ws_bytes < base + shape.desc_bytes + shape.part_bytes ||
-                    (double)shape.tiles * g.Hkv * ((double)g.max_blocks * g.bs / 32 + 2) >= 2147483648.0))
-    shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, false);
+                    (double)shape.tiles * g.Hkv * ((double)g.max_blocks * g.bs / 32 + 2 + kWideBegin) >= 2147483648.0))
+    shape = masked_shape(g.T, g.S, g.Hq, g.Hkv, g.D, m.kind, false);
   if (shape.tiles * g.Hkv >= (1L << 31)) return false;
   MaskedArgs a{};
   a.d.q = static_cast<const h16*>(m.q);
@@ -150,10 +159,10 @@ bool mfma(const Call& c, MfmaCall m, int* rc) {
     a.desc = reinterpret_cast<int4*>(p + shape.part_bytes);
   }
   switch (m.kind) {
-    case KvKind::f16: launch_masked_kind<KvF16>(a, m.D, shape.kw, c.st); break;
-    case KvKind::bf16: launch_masked_kind<KvBF16>(a, m.D, shape.kw, c.st); break;
-    case KvKind::fp8: launch_masked_kind<KvFp8>(a, m.D, shape.kw, c.st); break;
-    case KvKind::affine: launch_masked_affine(m, a, shape.kw, c.st); break;
+    case KvKind::f16: launch_masked_kind<KvF16>(a, m.D, shape.cw, c.st); break;
+    case KvKind::bf16: launch_masked_kind<KvBF16>(a, m.D, shape.cw, c.st); break;
+    case KvKind::fp8: launch_masked_kind<KvFp8>(a, m.D, shape.cw, c.st); break;
+    case KvKind::affine: launch_masked_affine(m, a, shape.cw, c.st); break;
   }
   *rc = entry_check_launch("masked_wide");
   return true;
@@ -170,9 +179,12 @@ size_t emx_masked_workspace_bytes(int num_tokens, int num_seqs, int num_q_heads,
   if (num_tokens <= 0 || num_seqs <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads ||
       !head_ok(head_dim))
     return 0;
-  const MaskedShape m = masked_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, true);
-  size_t part = m.desc_bytes + m.part_bytes;
-  if (num_tokens == num_seqs)
+  size_t part = 0;  // (whatever the cache)
+  for (const KvKind kind : {KvKind::f16, KvKind::fp8, KvKind::affine}) {
+    const MaskedShape m = masked_shape(num_tokens, num_seqs, num_q_heads, num_kv_heads, head_dim, kind, true);
+    part = std::max(part, m.desc_bytes + m.part_bytes);
+  }
+  if (num_tokens == num_seqs && num_q_heads / num_kv_heads <= kMaskedHeads)
     part = std::max(part, decode_mfma_partial_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim));
   return part ? workspace_base() + part : 0;
 }

@@ -60,16 +60,16 @@ struct MaskedArgs;  // masked_wide.hpp
 
 // How a call is cut (sizes and types only).
 struct MaskedShape {
-  int kw, tokb;       // key waves of a workgroup, query tokens of a tile (0: not taken)
+  int cw, tokb;       // column waves of a workgroup (32 columns each), query tokens of a tile (0: not taken)
   long tiles;         // the most tiles per kv head
   int wgs;            // workgroups over which tiles are cut, 0: they are not
   size_t desc_bytes, part_bytes;
 };
-MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, bool cut);
+MaskedShape masked_shape(int T, int S, int Hq, int Hkv, int D, KvKind kind, bool cut);
 
 // Single-token rows (c.qsl null) with a window and sinks > 0; buffers as launch_decode_mfma's (emx_masked_rows.hip).
 void launch_masked_rows(const MfmaCall& c, int sinks, int* ws_cnt, float* partials, hipStream_t st);
 
-void launch_masked_affine(const MfmaCall& c, const MaskedArgs& a, int kw, hipStream_t st);  // emx_masked_affine.hip
+void launch_masked_affine(const MfmaCall& c, const MaskedArgs& a, int cw, hipStream_t st);  // emx_masked_affine.hip
 
 }  // namespace emx

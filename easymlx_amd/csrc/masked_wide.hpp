@@ -14,13 +14,19 @@
 // backwards because a drafted node's ancestors then come in the order of its walk to the root: each
 // lane keeps one cursor, and a block of drafted keys costs as many steps as it holds ancestors, for
 // trees of any size.  Where a launch has tiles enough each is a workgroup's; else the blocks of all
-// tiles in a row are cut into equal ranges, one to a workgroup (WidePlan), and a tile that is not
-// inside one range leaves its parts' fp32 state to masked_merge, which joins them in part order.
+// tiles in a row (and what it costs to begin each, kWideBegin) are cut into equal ranges, one to a
+// workgroup, and a tile that is not inside one range leaves its parts' fp32 state to masked_merge,
+// which joins them in part order.
 //
-// A block: K and V are loaded once per workgroup, a block ahead into registers, and go to the other
-// of two LDS images as 16-bit values (FP8: dec(code) * 2^-8, exact; affine codes as exact
-// sub-normals), 16-byte chunks turned by the row so that operand reads touch every bank: one barrier
-// a block.  A wave has 32 columns (and, KW = 2, half of the block's keys), on v_mfma 32x32x16:
+// A block: K and V are read once per workgroup, a block ahead, into the other of two LDS images of
+// 16-bit values, 16-byte chunks turned by the row so that operand reads touch every bank: one barrier
+// a block.  fp16 / bf16 rows go there as they are, with no register between (a block's 32 registers
+// of a thread were spilled, and each reload waited for the loads themselves: 870 -> 745 us over 12
+// trees of 48 to 64 nodes with 64 / 8 heads and up to 32768 keys); FP8 (dec(code) * 2^-8, exact) and
+// affine codes (exact sub-normals) through registers.  A wave has 32 columns (KW = 2: and half of the
+// block's keys; D = 256: and half of the dims, the two halves of its scores meeting in LDS: a wave's
+// state then fits 256 registers, 83 -> 66 us over three prompt chunks on 8-bit pages), on v_mfma
+// 32x32x16:
 //   S^T : A = K rows, B = queries; a lane ends with half of its tile's scores of ONE column, so that
 //         maximum, reference and sum are its own, and lanes meet only where a score passes the
 //         reference by 2^kLazyMax;
@@ -28,6 +34,9 @@
 //         lane's own probabilities as two 16-bit parts, each the nearest (fp16: 22 bits of the 24; bf16:
 //         16, which puts an output off by at most 2^-17 of the largest value it averages: one part would
 //         add an error as large as the output's own rounding).
+// Bound: matrix instructions, 1.5 times the formula's for the second part, at the 1.27 PFLOP/s that a
+// large bf16 product reaches (those 12 trees: 543 us of the 745; without the loads 620); over affine
+// pages the vector unit (codes to values, scales, softmax: 480 instructions a block and wave).
 #pragma once
 
 #include "masked_launch.hpp"
@@ -71,46 +80,50 @@ struct MaskedArgs {
   int T;            // query rows
   int tiles;        // tiles per kv head, at most
   int wgs;          // > 0: tiles are cut, over at most that many workgroups; 0: a workgroup to a tile
-  int4* desc;       // cut: [1 + Hkv * tiles] {tiles of the launch}, then what masked_merge has to know of a tile
+  int4* desc;       // cut: [1 + min(Hkv * tiles, wgs)] {how many of them}, then what masked_merge has to know of a tile
   float* part;      // cut: [2 * wgs][part floats]
 };
 
+// What beginning a tile costs (pages, queries, first block; a part written), in blocks: 6 to 9 us against 2 to 3 us a block.
+// Ranges are equal with it: without, those of short tiles ended last.
+constexpr int kWideBegin = 3;
 // Fewest blocks of a workgroup's range; and how many blocks longer than an equal share the longest tile may be before
 // tiles are cut, where there is a workgroup for each (parts go to memory and back: 64 KiB each way, and a launch).
 constexpr int kWideRangeBlocks = 2;
 constexpr int kWideCutBlocks = 6;
+constexpr int kWideParts = 1024;   // more than a tile's parts
 constexpr int kWideTreeLds = 512;  // nodes of a tree whose parents are kept in LDS
 
-template <class C, int D, int KW>
+template <class C, int D, int KW, int CW>
 struct WideCfg {
   static constexpr int EB = sizeof(typename C::ET);
-  static constexpr int CW = 4 / KW;                 // waves side by side over the columns
-  static constexpr int COLS = 32 * CW;
+  static constexpr int DW = D > 128 ? 2 : 1;        // waves that share a column's dims
+  static constexpr int TH = 64 * KW * CW * DW;      // threads
   static constexpr int NT = D > 128 ? 32 * KW : 64; // keys of a block
   static constexpr int KT = NT / KW / 32;           // 32-key tiles of a wave's share of it
-  static constexpr int KS = D / 16;                 // QK^T k-slices
-  static constexpr int DT = D / 32;                 // PV dim tiles
-  static constexpr int G = 1;
+  static constexpr int KS = D / 16 / DW;            // QK^T k-slices of a wave
+  static constexpr int DT = D / 32 / DW;            // PV dim tiles
+  static constexpr int G = 1, GV = 1;               // quantization groups of a key, of a wave's dims
   static constexpr int PR = D * EB / 16;            // 16-byte pieces per row
-  static constexpr int NP = NT * PR / 256;          // pieces per thread and block, of K and of V
+  static constexpr int NP = NT * PR / TH;           // pieces per thread and block, of K and of V
   static constexpr int VB = NT * D * 2;             // bytes of the V image
   static constexpr int SCB = C::kFp8 ? 2 * 4 * NT : 0;  // of the scales
-  static_assert(KT >= 1 && NT * PR % 256 == 0, "whole 32-key tiles and pieces");
+  static_assert(KT >= 1 && NT * PR % TH == 0, "whole 32-key tiles and pieces");
 };
-template <int BITS, int GS, int D, int KW>
-struct WideCfg<KvAffine<BITS, GS>, D, KW> {
-  static constexpr int CW = 4 / KW, COLS = 32 * CW, NT = D > 128 ? 32 * KW : 64, KT = NT / KW / 32;
-  static constexpr int KS = D / 16, DT = D / 32, G = D / GS;
+template <int BITS, int GS, int D, int KW, int CW>
+struct WideCfg<KvAffine<BITS, GS>, D, KW, CW> {
+  static constexpr int DW = D > 128 ? 2 : 1, TH = 64 * KW * CW * DW, NT = D > 128 ? 32 * KW : 64, KT = NT / KW / 32;
+  static constexpr int KS = D / 16 / DW, DT = D / 32 / DW, G = D / GS, GV = G / DW;
   static constexpr int RBK = D * BITS / 8;              // bytes of a key's codes
   static constexpr int PR = RBK / 16;                   // 16-byte pieces of them
   static constexpr int NPK = NT * PR;                   // K pieces of a block
-  static constexpr int NP = (NPK + 255) / 256;
+  static constexpr int NP = (NPK + TH - 1) / TH;
   static constexpr int UT = 64 / BITS, U = NT / UT;     // V units: 8 bytes, UT tokens of one dim
-  static constexpr int NPV = D * U / 256;               // V units per thread
+  static constexpr int NPV = D * U / TH;                // V units per thread
   static constexpr int NPS = 4 * G * NT / 8;            // 16-byte scale pieces of a block
   static constexpr int VB = D * NT * 2;                 // [dim][NT], 16-byte chunks turned by v_turn
   static constexpr int SCB = 3 * 4 * G * NT + 16 * NT;  // ks, vs, vb [group][NT] floats, bias operand rows
-  static_assert(NPS <= 64 && D * U % 256 == 0, "one scale piece per lane, whole V units per thread");
+  static_assert(NPS <= 64 && D * U % TH == 0, "one scale piece per lane, whole V units per thread");
 };
 
 // Where 16-byte chunk c of a row stands in its row, so that the lanes that LDS serves in one cycle touch all 64 banks.
@@ -130,9 +143,28 @@ __device__ __forceinline__ constexpr int va_turn(const int dim, const int c) {
   return c ^ (NT == 64 ? (dim >> 1) & 7 : (dim >> 2) & 3);
 }
 
+// 16 bytes from `src` (each lane its own) to LDS byte `dst` + 16 lane, with no register between.  Nothing waits for it but
+// dma_wait: the compiler's own waits count only loads that it knows, which come back in order with these.  (By the
+// compiler's builtin every transposing LDS read that follows waits for it, in the block before the one it loads.)
+__device__ __forceinline__ void dma16(const void* src, const uint32_t dst) {
+  uint32_t m0;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0)
+               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(dst))
+               : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// The same value, as one that the compiler has not seen: what is computed from it inside a loop is computed there, and
+// takes no register (or, worse, scratch memory: its reload waits for every load issued before it) all through the loop.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // Floats of a part: per column wave DT * 4 + 1 vectors of 4 a lane.
-template <int D, int KW>
-constexpr int kWidePart = (4 / KW) * (D / 8 + 1) * 256;
+template <int D, int CW>
+constexpr int kWidePart = CW * (D / 8 + 1) * 256;
 
 // A tile's blocks: positions backwards from block `hi`, `n` in all, the last `sink` of them the blocks 0 .. sink - 1.
 struct MaskedSpan {
@@ -182,22 +214,24 @@ __device__ __forceinline__ int masked_blocks(const MaskedArgs& A, const MaskedSe
   return max(1, masked_span<NT>(A.mask, q.past, tile * A.tokb, masked_tok_hi(A, q, tile)).n);
 }
 
-// The sum over the workgroup of the threads before this one (256 threads; red: 8 ints of LDS); total: of all.
+// The sum over the workgroup of the threads before this one (NW waves; red: NW ints of LDS); total: of all.
+template <int NW>
 __device__ __forceinline__ int wg_scan(const int mine, int* red, int& total) {
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  int x = mine;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int y = __shfl_up(x, o, 64);
-    if (lane >= o) x += y;
-  }
+  int x = mine;  // within rows of 16 lanes, then over the rows before
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
   __syncthreads();  // (red may still be read)
   if (lane == 63) red[wv] = x;
   __syncthreads();
   int base = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < NW; ++w) {
     base += w < wv ? red[w] : 0;
     total += red[w];
   }
@@ -214,8 +248,9 @@ __device__ __forceinline__ MaskedSeq wide_seq(const MaskedArgs& A, const int* se
 }
 
 // tcum[s]: tiles of the sequences before s, tcum[S] of all; seqs: wide_seq's.
+template <int NW>
 __device__ __forceinline__ void wide_tiles(const MaskedArgs& A, int* tcum, int* seqs, int* red) {
-  const int S = A.d.S, ch = (S + 255) / 256, s0 = threadIdx.x * ch;
+  const int S = A.d.S, ch = (S + 64 * NW - 1) / (64 * NW), s0 = threadIdx.x * ch;
   int mine = 0, total;
   for (int i = 0; i < ch && s0 + i < S; ++i) {
     const MaskedSeq q = masked_seq(A, s0 + i);
@@ -228,7 +263,7 @@ __device__ __forceinline__ void wide_tiles(const MaskedArgs& A, int* tcum, int* 
       seqs[2 * kWideSeqLds + s0 + i] = q.past;
     }
   }
-  int run = wg_scan(mine, red, total);
+  int run = wg_scan<NW>(mine, red, total);
   for (int i = 0; i < ch && s0 + i < S; ++i) {
     const int n = tcum[s0 + i];
     tcum[s0 + i] = run;
@@ -318,6 +353,17 @@ __device__ void attend_masked(const DecodeArgs& a, const MaskRule& mask, const M
     if (lane + 64 * n >= d0 && lane + 64 * n < d1) from_f32(acc[n] * li, reinterpret_cast<QT*>(a.out) + ro + lane + 64 * n);
 }
 
+// Equal ranges of `all` blocks for n workgroups (all >= n): where range w begins, and whose block x is.
+struct WideRanges {
+  int q, r;
+  __device__ __forceinline__ WideRanges(const int all, const int n) : q(all / n), r(all - all / n * n) {}
+  __device__ __forceinline__ int begin(const int w) const { return w * q + min(w, r); }
+  __device__ __forceinline__ int owner(const int x) const {
+    const int big = r * (q + 1);
+    return x < big ? x / (q + 1) : r + (x - big) / q;
+  }
+};
+
 // Column c of a tile: which token and head; token -1 where there is none.
 __device__ __forceinline__ void masked_column(const MaskedArgs& A, const MaskedSeq& q, const int tile, const int c,
                                               const int HG, int& tok, int& head) {
@@ -353,30 +399,34 @@ __device__ __forceinline__ uint32_t below(const int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u;
 }
 
-// (Two workgroups to a compute unit where a wave's state fits 256 registers.)
-template <class C, int D, int KW>
-__global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 1)) ? 1 : 2) void masked_wide(MaskedArgs A) {
-  using P = WideCfg<C, D, KW>;
+// (256 registers a wave: two waves to a SIMD)
+template <class C, int D, int KW, int CW>
+__global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(MaskedArgs A) {
+  using P = WideCfg<C, D, KW, CW>;
   typedef typename C::Op Op;
   typedef typename C::QT QT;
   const DecodeArgs& a = A.d;
-  constexpr int NT = P::NT, KT = P::KT, KS = P::KS, DT = P::DT, G = P::G, CW = P::CW;
+  constexpr int NT = P::NT, KT = P::KT, KS = P::KS, DT = P::DT, G = P::G, GV = P::GV, TH = P::TH, NW = TH / 64;
   constexpr bool AFF = C::kAffine, FP8 = C::kFp8;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int cw = wv % CW, kw = wv / CW;  // this wave's columns, and its share of a block's keys
+  const int cw = wv % CW, kw = wv / CW % KW;    // this wave's columns, its share of a block's keys
+  const int dw = P::DW > 1 ? wv / (CW * KW) : 0;  // ... and of the dims
   const int c32 = lane & 31, half = lane >> 5;
 
-  // ---- LDS: tables, then two images of a block (K rows, V, scales); the states of a unit's key waves meet there too
-  constexpr int oTc = 0, oSeq = lds_next(oTc, 4 * (kWideSeqs + 1));
-  constexpr int oPar = lds_next(oSeq, 12 * kWideSeqLds), oRed = lds_next(oPar, 4 * kWideTreeLds);
-  constexpr int oBuf = (lds_next(oRed, 128) + 511) & ~511;
-  constexpr int KB = NT * D * 2, oV = KB, oSc = oV + P::VB, BUF = (oSc + P::SCB + 16 + 511) & ~511;
+  // ---- LDS: two images of a block (K rows, V, scales; the states of a unit's key waves meet there too), then tables
+  constexpr bool DMA = !AFF && !FP8;  // rows go to the images as they are: no register between
+  constexpr int oBuf = 0, KB = NT * D * 2, oV = KB, oSc = oV + P::VB;
+  constexpr int BUF = (oSc + (DMA ? 0 : P::SCB + 16) + 511) & ~511;
   static_assert(KB % 512 == 0 && P::VB % 512 == 0, "the images' chunks are flipped by address bits");
+  static_assert(!DMA || 2 * BUF <= 65536, "where dma16 may write: its LDS address has 16 bits");
   constexpr int MEET = KW > 1 ? CW * (4 * DT + 1) * 64 * 16 : 0;
-  constexpr int oEnd = oBuf + (2 * BUF > MEET ? 2 * BUF : MEET);
-  static_assert(oEnd <= 81920, "two workgroups to a compute unit");
+  constexpr int oTc = 2 * BUF > MEET ? 2 * BUF : MEET, oSeq = lds_next(oTc, 4 * (kWideSeqs + 1));
+  constexpr int oPar = lds_next(oSeq, 12 * kWideSeqLds), oRed = lds_next(oPar, 4 * kWideTreeLds);
+  constexpr int oX = lds_next(oRed, 128);  // two waves to a column's dims: a wave's part of its scores
+  constexpr int oEnd = oX + (P::DW > 1 ? TH * KT * 64 : 0);
+  static_assert(oEnd <= (TH > 256 ? 163840 : 81920), "256 threads: two workgroups to a compute unit");
   __shared__ __attribute__((aligned(512))) unsigned char lds[oEnd];
   int* tcum = reinterpret_cast<int*>(lds + oTc);
   int* seqs = reinterpret_cast<int*>(lds + oSeq);
@@ -385,36 +435,41 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
 
   const MaskRule mask = A.mask;
   const int HG = a.Hq / a.Hkv, S = a.S;
-  if (a.qsl) {
-    const int lo = a.qsl[0], hi = a.qsl[S];
-    if (lo > 0 || hi < A.T) zero_other_rows<QT>(a, A.T, D, blockIdx.x, gridDim.x);
-  }
+  const int row_lo = a.qsl ? a.qsl[0] : 0, row_hi = a.qsl ? a.qsl[S] : A.T;
 
-  // ---- this workgroup's range [at, end) of the blocks of all tiles, kv head by kv head
-  wide_tiles(A, tcum, seqs, red);
+  bool first_seg = true;
+  const bool by_tile = a.Hkv * A.tiles <= A.wgs;
+  int4 cut_tile{0, 0, 0, 0};  // for masked_merge: the tile whose first block this range has, and not its last
+
+  // ---- this workgroup's range [at, end) of the units of all tiles, kv head by kv head: kWideBegin to begin a tile, then
+  // its blocks
+  wide_tiles<NW>(A, tcum, seqs, red);
+  if (row_lo > 0 || row_hi < A.T) zero_other_rows<QT>(a, A.T, D, blockIdx.x, gridDim.x);
   const int ntiles = __builtin_amdgcn_readfirstlane(tcum[S]);
-  int kvh, t, b0, todo, w = 0, nwg = 0, all = 0;  // kv head, tile, block within it, blocks left; nwg 0: no tile is cut
+  int kvh, t, u0, todo, w = 0, nwg = 0;  // kv head, tile, unit within it, units left; nwg 0: no tile is cut
+  WideRanges ranges(0, 1);
   if (A.wgs == 0) {
     kvh = blockIdx.x % a.Hkv;
     t = ntiles - 1 - (int)blockIdx.x / a.Hkv;  // (the longest of a sequence first)
-    b0 = 0;
+    u0 = 0;
     todo = 0x7FFFFFFF;
     if (t < 0) return;
   } else {
-    const int ch = (ntiles + 255) / 256, t0 = tid * ch;
+    const int ch = (ntiles + TH - 1) / TH, t0 = tid * ch;
     int mine = 0, most = 0, per;
     for (int i = 0, s = 0; i < ch && t0 + i < ntiles; ++i) {
       if (i == 0) s = wide_seq_of(tcum, S, t0);
       while (tcum[s + 1] <= t0 + i) ++s;
-      const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]);
+      const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]) + kWideBegin;
       mine += n;
       most = max(most, n);
     }
     most = (int)wave_max((float)most);
-    if (lane == 0) red[4 + wv] = most;
-    const int before = wg_scan(mine, red, per);
-    most = max(max(red[4], red[5]), max(red[6], red[7]));
-    all = per * a.Hkv;  // (the host keeps it below 2^31)
+    if (lane == 0) red[8 + wv] = most;
+    const int before = wg_scan<NW>(mine, red, per);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) most = max(most, red[8 + i]);
+    const int all = per * a.Hkv;  // (the host keeps it below 2^31)
     nwg = min(A.wgs, max(1, all / kWideRangeBlocks));
     if (nwg >= 8) nwg &= ~7;
     const int nt = ntiles * a.Hkv;
@@ -424,48 +479,49 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
       if ((int)blockIdx.x >= nt) return;
       kvh = blockIdx.x % a.Hkv;
       t = blockIdx.x / a.Hkv;
-      b0 = 0;
+      u0 = 0;
       todo = 0x7FFFFFFF;
     } else {
     if ((int)blockIdx.x >= nwg) return;
     // workgroups of one XCD (blockIdx mod 8) take neighbouring ranges: tiles of one sequence and kv head share its L2
     w = nwg >= 8 ? (int)(blockIdx.x % 8) * (nwg / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
-    const int at = (int)((long long)w * all / nwg);
-    todo = (int)((long long)(w + 1) * all / nwg) - at;
+    ranges = WideRanges(all, nwg);
+    const int at = ranges.begin(w);
+    todo = ranges.begin(w + 1) - at;
     kvh = at / per;
     const int r = at - kvh * per;
     if (r >= before && r < before + mine) {  // one thread's tiles hold it
       int x = before, i = 0, s = wide_seq_of(tcum, S, t0);
       for (;; ++i) {
         while (tcum[s + 1] <= t0 + i) ++s;
-        const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]);
+        const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]) + kWideBegin;
         if (r < x + n) break;
         x += n;
       }
-      red[8] = t0 + i;
-      red[9] = r - x;
+      red[16] = t0 + i;
+      red[17] = r - x;
     }
-    if (blockIdx.x == 0 && tid == 0) A.desc[0] = int4{ntiles, 0, 0, 0};
+    if (blockIdx.x == 0 && tid == 0) A.desc[0] = int4{by_tile ? ntiles : nwg, 0, 0, 0};
     __syncthreads();
-    t = __builtin_amdgcn_readfirstlane(red[8]);
-    b0 = __builtin_amdgcn_readfirstlane(red[9]);
+    t = __builtin_amdgcn_readfirstlane(red[16]);
+    u0 = __builtin_amdgcn_readfirstlane(red[17]);
     }
   }
 
   // ---- lane constants of the operand reads (image-relative bytes; the images start at multiples of 512)
-  const int kad = (kw * KT * 32 + c32) * (D * 2) + (k_turn<D>(c32, half) << 4);  // K: row c32 (+ 32 per tile), chunk 2 w + half
+  const int kad = (kw * KT * 32 + c32) * (D * 2) + (k_turn<D>(c32, KS * 2 * dw + half) << 4);  // K: row c32 (+ 32 per tile), chunk 2 w + half
   int vad;  // V: 4 tokens of 16 dims per 16 lanes, chunk 4 d + ..; affine: dim c32 (+ 32 per tile), chunk 4 kt + 2 j + half
   if constexpr (AFF) {
-    vad = oV + c32 * (NT * 2) + (va_turn<NT>(c32, kw * KT * 4 + half) << 4);
+    vad = oV + (dw * DT * 32 + c32) * (NT * 2) + (va_turn<NT>(c32, kw * KT * 4 + half) << 4);
   } else {
     const int i = lane & 15, row = 4 * half + (i >> 2), c = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-    vad = oV + (kw * KT * 32 + row) * (D * 2) + (v_turn<D>(row, c) << 4) + (i & 1) * 8;
+    vad = oV + (kw * KT * 32 + row) * (D * 2) + (v_turn<D>(row, c + 4 * DT * dw) << 4) + (i & 1) * 8;
   }
   const float sl2 = a.scale_log2;
   const size_t rowb = (size_t)a.Hkv * D * sizeof(typename C::ET);  // token-major
   typedef __attribute__((address_space(3))) unsigned char* lptr;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr)lds;
 
-  bool first_seg = true;
   int sidx = wide_seq_of(tcum, S, t);
   for (;;) {
     // ---- a segment: blocks [b0, b1) of tile t
@@ -478,16 +534,13 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
     const int q0 = sq.q0, past = sq.past;
     const int tok_lo = tile * A.tokb, tok_hi = masked_tok_hi(A, sq, tile);
     const MaskedSpan span = masked_span<NT>(mask, past, tok_lo, tok_hi);
-    const int nblk = max(1, span.n), b1 = min(nblk, b0 + min(todo, nblk - b0));
+    const int nblk = max(1, span.n), u1 = min(nblk + kWideBegin, u0 + min(todo, nblk + kWideBegin - u0));
+    const int b0 = max(0, u0 - kWideBegin), b1 = max(0, u1 - kWideBegin);
+    if (b0 < b1) {
     const int st_lo = b0, st_hi = min(b1, span.n);  // (an empty tile has a block of nothing)
     const int k_hi = max(past + tok_hi, 0);
     const int32_t* par = mask.parents ? mask.parents + q0 : nullptr;
     const bool tree = par != nullptr, tree_lds = tree && sq.qlen <= kWideTreeLds;
-    __syncthreads();  // (the last segment's LDS is free)
-    if (tree_lds) {
-      for (int i = tid; i <= tok_hi; i += 256) lpar[i] = parent_of(par, i);
-      __syncthreads();
-    }
     auto up = [&](const int i) { return tree_lds ? lpar[i] : parent_of(par, i); };
     auto pos_of_block = [&](const int st) {
       const int lo = span.n - span.sink;
@@ -501,12 +554,13 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
     auto page_id = [&](const int st) {
       return bt[page_of(min(pos_of_block(st) + (lane & (NT - 1)), k_hi), A.inv_bs)];
     };
-    u32x4 rk[P::NP], rv[AFF ? 1 : P::NP];  // the next block's pieces
+    u32x4 rk[P::NP], rv[AFF ? 1 : P::NP];  // the next block's pieces (DMA: none)
     u32x2 ru[AFF ? 16 : 1];                // affine: its V units
     u32x4 rs;                              // affine, wave 0: scale piece `lane`
     uint64_t okn = 0;                      // keys of that block on a valid page
     float psk = 0.f, psv = 0.f;            // FP8: page scales of key `lane` of that block
-    auto load_block = [&](const int st, const int blk) {
+    auto load_block = [&](const int st, const int blk, const int buf) {
+      const unsigned tid = anew(threadIdx.x), lane = tid & 63;
       const int pos = min(pos_of_block(st) + (lane & (NT - 1)), k_hi);
       const bool ok = (unsigned)blk < (unsigned)a.nb;
       okn = __ballot(ok);
@@ -516,7 +570,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
         constexpr int B = C::kBits;
         const int row = (b * a.Hkv + kvh) * a.bs + off;
         if (wv == 0) {
-          const int pc = min(lane, P::NPS - 1), seg = pc / (NT / 8), arr = seg / G, g = seg % G;
+          const int pc = min((int)lane, P::NPS - 1), seg = pc / (NT / 8), arr = seg / G, g = seg % G;
           const int r8 = __shfl(row, 8 * (pc % (NT / 8)), 64), o8 = __shfl(off, 8 * (pc % (NT / 8)), 64);
           const h16 *b_ks = a.ks, *b_kb = a.kb, *b_vs = a.vs, *b_vb = a.vb;
           asm("" : "+s"(b_ks), "+s"(b_kb), "+s"(b_vs), "+s"(b_vb));  // picked from registers, not by a vector load
@@ -526,20 +580,16 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
           rs = *(gu32x4)(base + (size_t)G * (r8 - o8) + (size_t)g * a.bs + (o8 & ~7));
         }
 #pragma unroll
-        for (int n = 0; n < P::NP; ++n) {
-          const int e = tid + 256 * n;  // (fewer than 256 pieces: the others repeat them)
-          const int r = __shfl(row, (e / P::PR) & (NT - 1), 64);
-          rk[n] = *reinterpret_cast<const u32x4*>(kbase + (size_t)r * P::RBK + 16 * (e % P::PR));
+        for (int n = 0; n < P::NP; ++n) {  // (fewer pieces than threads: the others repeat them)
+          const int r = __shfl(row, (tid / P::PR + n * (TH / P::PR)) & (NT - 1), 64);
+          rk[n] = *reinterpret_cast<const u32x4*>(kbase + (size_t)r * P::RBK + 16 * (tid % P::PR));
         }
         const int T = min(a.bs, 256 / B);  // tokens of a value tile (a power of two)
+        const int r = __shfl(row, tid % P::U * P::UT, 64), o = (r & (T - 1)) & ~(P::UT - 1);
+        const uint32_t* vu = reinterpret_cast<const uint32_t*>(vbase) + (size_t)(r & ~(T - 1)) * (D * B / 32) +
+                             ((int)(tid / P::U) * T + o) * B / 32;
 #pragma unroll
-        for (int n = 0; n < P::NPV; ++n) {
-          const int e = tid + 256 * n, uu = e % P::U, dim = e / P::U;
-          const int r = __shfl(row, uu * P::UT, 64);
-          const int o = (r & (T - 1)) & ~(P::UT - 1);
-          ru[n] = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint32_t*>(vbase) +
-                                                  (size_t)(r & ~(T - 1)) * (D * B / 32) + (dim * T + o) * B / 32);
-        }
+        for (int n = 0; n < P::NPV; ++n) ru[n] = *reinterpret_cast<const u32x2*>(vu + n * (TH / P::U) * T * B / 32);
       } else {
         const int row = b * a.bs + off;
         if constexpr (FP8) {
@@ -548,49 +598,59 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
         }
 #pragma unroll
         for (int n = 0; n < P::NP; ++n) {
-          const size_t o = (size_t)__shfl(row, tid / P::PR + n * (256 / P::PR), 64) * rowb + 16 * (tid % P::PR);
-          rk[n] = *reinterpret_cast<const u32x4*>(kbase + o);
-          rv[n] = *reinterpret_cast<const u32x4*>(vbase + o);
+          const int r = tid / P::PR + n * (TH / P::PR), c = (int)(tid % P::PR);
+          const size_t o = (size_t)__shfl(row, r, 64) * rowb;
+          if constexpr (DMA) {  // a wave's 64 pieces stand in a row in the image: each lane takes the chunk that belongs there
+            const uint32_t dst = lds0 + oBuf + buf * BUF + (wv + n * (TH / 64)) * 1024;
+            dma16(kbase + o + 16 * k_turn<D>(r, c), dst);
+            dma16(vbase + o + 16 * v_turn<D>(r, c), dst + oV);
+          } else {
+            rk[n] = *reinterpret_cast<const u32x4*>(kbase + o + 16 * c);
+            rv[n] = *reinterpret_cast<const u32x4*>(vbase + o + 16 * c);
+          }
         }
       }
     };
     // ... and their way to image `buf`, once they are here.  vex: the exponent that the value scales of the images carry
     int vex = 0;
     auto store_block = [&](const int st, const int buf) {
+      const unsigned tid = anew(threadIdx.x), lane = tid & 63;
       unsigned char* img = lds + oBuf + buf * BUF;
       if constexpr (AFF) {
         constexpr int B = C::kBits;
+        // (chunk numbers are multiples of the chunks of a piece or unit: the next ones stand at flipped address bits; the
+        // rows of a thread's next piece or unit are turned as its first's)
+        static_assert(TH / P::PR % 16 == 0 && TH / P::U % 16 == 0, "turned alike");
+        const int kr0 = (tid / P::PR) & (NT - 1), ka0 = kr0 * (D * 2) + (k_turn<D>(kr0, tid % P::PR * (16 / B)) << 4);
 #pragma unroll
         for (int n = 0; n < P::NP; ++n) {
-          const int e = tid + 256 * n, row = (e / P::PR) & (NT - 1), c0 = (e % P::PR) * (16 / B);
-          unsigned char* kr = img + row * (D * 2);
-          if (e < P::NPK) {
+          unsigned char* kr = img + n * (TH / P::PR) * (D * 2);
+          if (P::NPK >= TH || tid < P::NPK) {
             if constexpr (B == 4) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<h16x8*>(kr + (k_turn<D>(row, c0 + i) << 4)) = unpack4_high(rk[n][i]);
+              for (int i = 0; i < 4; ++i) *reinterpret_cast<h16x8*>(kr + (ka0 ^ (i << 4))) = unpack4_high(rk[n][i]);
             } else {
 #pragma unroll
               for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<h16x8*>(kr + (k_turn<D>(row, c0 + i) << 4)) = unpack8(rk[n][2 * i], rk[n][2 * i + 1]);
+                *reinterpret_cast<h16x8*>(kr + (ka0 ^ (i << 4))) = unpack8(rk[n][2 * i], rk[n][2 * i + 1]);
             }
           }
         }
         // values: a dim's 16 tokens stand as 0-3, 8-11 and 4-7, 12-15: one read has a lane's eight
+        const int dim = tid / P::U, uu = tid % P::U;
+        const int va0 = dim * (NT * 2) + (va_turn<NT>(dim, B == 4 ? 2 * uu : uu & ~1) << 4) + (B == 4 ? 0 : 8 * (uu & 1));
 #pragma unroll
         for (int n = 0; n < P::NPV; ++n) {
-          const int e = tid + 256 * n, dim = e / P::U, uu = e % P::U;
-          unsigned char* vr = img + oV + dim * (NT * 2);
+          unsigned char* vr = img + oV + n * (TH / P::U) * (NT * 2);
           if constexpr (B == 4) {
             const u32x4 x = __builtin_bit_cast(u32x4, unpack4_high(ru[n][0]));
             const u32x4 y = __builtin_bit_cast(u32x4, unpack4_high(ru[n][1]));
-            *reinterpret_cast<u32x4*>(vr + 16 * va_turn<NT>(dim, 2 * uu)) = u32x4{x[0], x[1], y[0], y[1]};
-            *reinterpret_cast<u32x4*>(vr + 16 * va_turn<NT>(dim, 2 * uu + 1)) = u32x4{x[2], x[3], y[2], y[3]};
+            *reinterpret_cast<u32x4*>(vr + va0) = u32x4{x[0], x[1], y[0], y[1]};
+            *reinterpret_cast<u32x4*>(vr + (va0 ^ 16)) = u32x4{x[2], x[3], y[2], y[3]};
           } else {  // (a unit is the first or the second half of its 16)
             const u32x4 x = __builtin_bit_cast(u32x4, unpack8(ru[n][0], ru[n][1]));
-            const int c = uu & ~1, h8 = 8 * (uu & 1);
-            *reinterpret_cast<u32x2*>(vr + 16 * va_turn<NT>(dim, c) + h8) = u32x2{x[0], x[1]};
-            *reinterpret_cast<u32x2*>(vr + 16 * va_turn<NT>(dim, c + 1) + h8) = u32x2{x[2], x[3]};
+            *reinterpret_cast<u32x2*>(vr + va0) = u32x2{x[0], x[1]};
+            *reinterpret_cast<u32x2*>(vr + (va0 ^ 16)) = u32x2{x[2], x[3]};
           }
         }
         if (wv == 0) {
@@ -598,7 +658,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
           float *vsf = ksf + G * NT, *vbf = vsf + G * NT;
           h16* kbe = reinterpret_cast<h16*>(vbf + G * NT);
           // scales of keys past the tile's last one or on an invalid page (which may hold anything) as zeros
-          const int pc = min(lane, P::NPS - 1), t8 = 8 * (pc % (NT / 8)), seg = pc / (NT / 8), arr = seg / G,
+          const int pc = min((int)lane, P::NPS - 1), t8 = 8 * (pc % (NT / 8)), seg = pc / (NT / 8), arr = seg / G,
                     g = seg % G;
           const int live = k_hi + 1 - pos_of_block(st) - t8;
           u32x4 x = rs;
@@ -633,56 +693,58 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
             }
           }
         }
+      } else if constexpr (DMA) {
+        dma_wait();
       } else {
+        static_assert(TH / P::PR % 16 == 0, "a thread's next rows are turned as its first");
+        const int row = tid / P::PR, c = tid % P::PR * 2;
+        const int ka0 = row * (D * 2) + (k_turn<D>(row, c) << 4), va0 = oV + row * (D * 2) + (v_turn<D>(row, c) << 4);
 #pragma unroll
         for (int n = 0; n < P::NP; ++n) {
-          const int row = tid / P::PR + n * (256 / P::PR), c = (tid % P::PR) * (16 / P::EB / 8);
-          unsigned char* kr = img + row * (D * 2);
-          unsigned char* vr = kr + oV;
-          if constexpr (FP8) {
+          unsigned char* rows = img + n * (TH / P::PR) * (D * 2);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              auto wide8 = [&](const u32x4 x) {
-                return as_h8(e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e], 0x0C010C00u)),
-                             e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e], 0x0C030C02u)),
-                             e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e + 1], 0x0C010C00u)),
-                             e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e + 1], 0x0C030C02u)));
-              };
-              *reinterpret_cast<h16x8*>(kr + (k_turn<D>(row, c + e) << 4)) = wide8(rk[n]);
-              *reinterpret_cast<h16x8*>(vr + (v_turn<D>(row, c + e) << 4)) = wide8(rv[n]);
-            }
-          } else {
-            *reinterpret_cast<u32x4*>(kr + (k_turn<D>(row, c) << 4)) = rk[n];
-            *reinterpret_cast<u32x4*>(vr + (v_turn<D>(row, c) << 4)) = rv[n];
+          for (int e = 0; e < 2; ++e) {
+            auto wide8 = [&](const u32x4 x) {
+              return as_h8(e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e], 0x0C010C00u)),
+                           e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e], 0x0C030C02u)),
+                           e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e + 1], 0x0C010C00u)),
+                           e4m3x2_to_h16x2(__builtin_amdgcn_perm(0u, x[2 * e + 1], 0x0C030C02u)));
+            };
+            *reinterpret_cast<h16x8*>(rows + (ka0 ^ (e << 4))) = wide8(rk[n]);
+            *reinterpret_cast<h16x8*>(rows + (va0 ^ (e << 4))) = wide8(rv[n]);
           }
         }
-        if constexpr (FP8) {
-          if (wv == 0) {
-            // value scales enter with the probabilities, brought near 1 by a power of two that the accumulator carries
-            const float vmax = wave_max(psv);
-            const int ex = min(max((int)((__float_as_uint(vmax) >> 23) & 0xFFu) - 127, -60), 60);
-            if (ex > vex || ex < vex - 6) vex = ex;
-            if (lane == 0) *reinterpret_cast<int*>(img + oSc + P::SCB) = vex;
-            float* ksf = reinterpret_cast<float*>(img + oSc);
-            if (lane < NT) {
-              ksf[lane] = psk * 256.f;
-              ksf[NT + lane] = psv * __uint_as_float((uint32_t)(127 - vex) << 23);
-            }
+        if (wv == 0) {
+          // value scales enter with the probabilities, brought near 1 by a power of two that the accumulator carries
+          const float vmax = wave_max(psv);
+          const int ex = min(max((int)((__float_as_uint(vmax) >> 23) & 0xFFu) - 127, -60), 60);
+          if (ex > vex || ex < vex - 6) vex = ex;
+          if (lane == 0) *reinterpret_cast<int*>(img + oSc + P::SCB) = vex;
+          float* ksf = reinterpret_cast<float*>(img + oSc);
+          if (lane < NT) {
+            ksf[lane] = psk * 256.f;
+            ksf[NT + lane] = psv * __uint_as_float((uint32_t)(127 - vex) << 23);
           }
         }
       }
     };
 
-    int blk1 = 0;
+    int blk0 = 0, blk1 = 0;
     if (st_lo < st_hi) {
-      load_block(st_lo, page_id(st_lo));
+      blk0 = page_id(st_lo);
       blk1 = page_id(min(st_lo + 1, st_hi - 1));
     }
+    __syncthreads();  // (the last segment's LDS is free)
+    if (tree_lds) {
+      for (int i = tid; i <= tok_hi; i += TH) lpar[i] = parent_of(par, i);
+      __syncthreads();
+    }
+    if (st_lo < st_hi) load_block(st_lo, blk0, 0);
 
     // ---- this lane's column
     int tok, head;
     masked_column(A, sq, tile, cw * 32 + c32, HG, tok, head);
-    const bool busy = __any(tok >= 0);
+    const bool busy = P::DW > 1 || __any(tok >= 0);  // (waves that meet in a block all take part)
     int cur = tree ? tok : -1, back = 0;  // tree: the cursor, and how many steps above the column's node it is
     int depth = 0;
     if (tree && mask.window > 0)
@@ -705,8 +767,8 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
     {
       const bool ok = tok >= 0;
       const QT* qp = reinterpret_cast<const QT*>(a.q) +
-                     ((size_t)(ok ? q0 + tok : 0) * a.Hq + (size_t)kvh * HG + (ok ? head : 0)) * D + 8 * half;
-      float gsum[G] = {};
+                     ((size_t)(ok ? q0 + tok : 0) * a.Hq + (size_t)kvh * HG + (ok ? head : 0)) * D + 16 * KS * dw + 8 * half;
+      float gsum[GV] = {};
 #pragma unroll
       for (int w2 = 0; w2 < KS; ++w2) {
         const u32x4 x = *reinterpret_cast<const u32x4*>(qp + 16 * w2);
@@ -715,7 +777,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             qB[w2][i] = v[slot_perm<C::kBits>(i)];  // the unpacked codes' order
-            gsum[w2 * G / KS] += (float)v[i];
+            gsum[w2 * GV / KS] += (float)v[i];
           }
         } else {
           qB[w2] = v;
@@ -724,9 +786,9 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
       if constexpr (AFF) {
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          const float x = gsum[g] + __shfl_xor(gsum[g], 32, 64);
+          const float x = gsum[g % GV] + __shfl_xor(gsum[g % GV], 32, 64);
           const h16 hi = (h16)x;
-          if (half == 0) {
+          if (half == 0 && g / GV == dw) {
             qbias[2 * g] = hi;
             qbias[2 * g + 1] = (h16)(x - (float)hi);
           }
@@ -736,7 +798,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
 
     float m_run = -INFINITY, l_part = 0.f;
     f32x16 acc[DT];
-    float pb[G] = {};  // affine: sum p * v_bias
+    float pb[GV] = {};  // affine: sum p * v_bias
     int vexp = 0;      // FP8, affine: acc holds the sum / 2^vexp
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -744,7 +806,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
     if constexpr (AFF) {  // the bias operand's unused halves stay zero
-      for (int i = tid; i < 2 * NT; i += 256)
+      for (int i = tid; i < 2 * NT; i += TH)
         *reinterpret_cast<u32x4*>(lds + oBuf + (i / NT) * BUF + oSc + 12 * G * NT + 16 * (i % NT)) = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
     }
@@ -755,7 +817,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
       const int buf = (st - st_lo) & 1;
       const uint64_t okm = okn;
       if (st + 1 < st_hi) {
-        load_block(st + 1, blk1);
+        load_block(st + 1, blk1, buf ^ 1);
         blk1 = page_id(min(st + 2, st_hi - 1));
       }
       const unsigned char* img = lds + oBuf + buf * BUF;
@@ -786,176 +848,183 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
             return __builtin_bit_cast(Op, u32x4{v0[0], v0[1], v1[0], v1[1]});
           }
         };
+        // ---- S^T, 32 keys at a time, from the last backwards as the cursors go: element i is key 8 (i / 4) + 4 half + i % 4.
         // Operands are read ahead of the products that take them, held in that order by the barriers (the compiler
         // put each read right before its use: a wait of the whole LDS latency per product)
         constexpr int KA = KS < 4 ? KS : 4;  // K operands read ahead
         Op ka[KA];
 #pragma unroll
         for (int i = 0; i < KA; ++i) ka[i] = read_k(KT - 1, i);
+        f32x16 sc[KT];
 #pragma unroll
-        for (int kk = 0; kk < KT; ++kk) {
-          const int kt = KT - 1 - kk;  // backwards, as the cursors go; 32 keys at a time: their scores alone are in registers
-          const int k0 = (kw * KT + kt) * 32;
+        for (int kt = KT - 1; kt >= 0; --kt) {
           __builtin_amdgcn_sched_barrier(0);
-          // ---- S^T: element i is key 8 (i / 4) + 4 half + i % 4 of the 32
-          f32x16 sc;
+          const int k0 = (kw * KT + kt) * 32;
+          f32x16 c;
+          auto clear = [&]() {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+            for (int i = 0; i < 16; ++i) c[i] = 0.f;
+          };
+          auto product = [&](const int w2) {
+            c = mfma32(ka[w2 % KA], qB[w2], c);
+            if (w2 + KA < KS) ka[w2 % KA] = read_k(kt, w2 + KA);
+            else if (kt > 0) ka[w2 % KA] = read_k(kt - 1, w2 + KA - KS);
+          };
+          clear();
           if constexpr (AFF) {
             const h16* kbe = reinterpret_cast<const h16*>(ksf + 3 * G * NT);
-            sc = mfma32(*reinterpret_cast<const Op*>(kbe + 8 * (k0 + c32)), qbias, sc);
+            sc[kt] = mfma32(*reinterpret_cast<const Op*>(kbe + 8 * (k0 + c32)), qbias, c);
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              f32x16 c;
+            for (int g = 0; g < GV; ++g) {
+              clear();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) c[i] = 0.f;
-#pragma unroll
-              for (int w2 = g * KS / G; w2 < (g + 1) * KS / G; ++w2)
-                c = mfma32(w2 < KA ? ka[w2 < KA ? w2 : 0] : read_k(kt, w2), qB[w2], c);
+              for (int w2 = g * KS / GV; w2 < (g + 1) * KS / GV; ++w2) product(w2);
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const f32x4 ks4 = *reinterpret_cast<const f32x4*>(ksf + g * NT + k0 + 8 * j + 4 * half);
+                const f32x4 ks4 = *reinterpret_cast<const f32x4*>(ksf + (GV * dw + g) * NT + k0 + 8 * j + 4 * half);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sc[4 * j + r] = fmaf(c[4 * j + r], ks4[r], sc[4 * j + r]);
+                for (int r = 0; r < 4; ++r) sc[kt][4 * j + r] = fmaf(c[4 * j + r], ks4[r], sc[kt][4 * j + r]);
               }
+              __builtin_amdgcn_sched_barrier(0);  // (the scales' reads stay with their group)
             }
           } else {
 #pragma unroll
-            for (int w2 = 0; w2 < KS; ++w2)
-              sc = mfma32(w2 < KA ? ka[w2 < KA ? w2 : 0] : read_k(kt, w2), qB[w2], sc);
+            for (int w2 = 0; w2 < KS; ++w2) product(w2);
+            sc[kt] = c;
             if constexpr (FP8) {
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const f32x4 ks4 = *reinterpret_cast<const f32x4*>(ksf + k0 + 8 * j + 4 * half);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sc[4 * j + r] *= ks4[r];
+                for (int r = 0; r < 4; ++r) sc[kt][4 * j + r] *= ks4[r];
               }
             }
           }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (P::DW > 1) {  // the other half of the dims
+          f32x4* mine = reinterpret_cast<f32x4*>(lds + oX) + wv * (KT * 256) + lane;
+          const f32x4* other = reinterpret_cast<f32x4*>(lds + oX) + (wv ^ (CW * KW)) * (KT * 256) + lane;
+#pragma unroll
+          for (int i = 0; i < 4 * KT; ++i) {
+            const f32x16& x = sc[i / 4];
+            mine[i * 64] = f32x4{x[i % 4 * 4], x[i % 4 * 4 + 1], x[i % 4 * 4 + 2], x[i % 4 * 4 + 3]};
+          }
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < 4 * KT; ++i) {
+            const f32x4 y = other[i * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sc[i / 4][i % 4 * 4 + r] += y[r];
+          }
+        }
 
-          // ---- mask, where some key is not visible to every column of the wave
-          const int kp = pos_of_block(st) + k0;
-          const uint32_t okw = (uint32_t)(okm >> k0);
-          const bool drafted = tree && kp + 32 > past;
-          const bool full = !drafted && kp + 31 <= lim_lo && (kp >= start_hi || kp + 32 <= mask.sinks) &&
-                            okw == 0xFFFFFFFFu;
-          if (!full) {
-            // bit k: the column sees key kp + k
-            uint32_t see = below(limit + 1 - kp) & (~below(start - kp) | below(mask.sinks - kp));
+        // ---- mask, where some key is not visible to every column of the wave
+        const int kp = pos_of_block(st) + kw * KT * 32;
+        const uint64_t okw = okm >> (kw * KT * 32);
+        constexpr uint64_t kAll = KT == 2 ? ~0ull : 0xFFFFFFFFull;
+        const bool drafted = tree && kp + 32 * KT > past;
+        const bool full = !drafted && kp + 32 * KT - 1 <= lim_lo && (kp >= start_hi || kp + 32 * KT <= mask.sinks) &&
+                          (okw & kAll) == kAll;
+        if (!full) {
+#pragma unroll
+          for (int kt = KT - 1; kt >= 0; --kt) {
+            // bit k: the column sees key k1 + k
+            const int k1 = kp + 32 * kt;
+            uint32_t see = below(limit + 1 - k1) & (~below(start - k1) | below(mask.sinks - k1));
             if (drafted) {
-              while (cur >= 0 && past + cur >= kp) {
-                const int b = past + cur - kp;
+              while (cur >= 0 && past + cur >= k1) {
+                const int b = past + cur - k1;
                 if (b < 32 && (mask.window <= 0 || back < mask.window || place - back < mask.sinks)) see |= 1u << b;
                 cur = up(cur);
                 ++back;
               }
             }
-            see = (see & okw) >> (4 * half);
+            see = (see & (uint32_t)(okw >> (32 * kt))) >> (4 * half);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] = (see >> (8 * (i / 4) + i % 4)) & 1u ? sc[i] : -INFINITY;
+            for (int i = 0; i < 16; ++i) sc[kt][i] = (see >> (8 * (i / 4) + i % 4)) & 1u ? sc[kt][i] : -INFINITY;
           }
+        }
 
-          // ---- online softmax: the lane's own scores of its column
-          float top = -INFINITY;
+        // ---- online softmax: the lane's own scores of its column
+        float top = -INFINITY;
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, sc[i]), sc[i + 1]);
-          if (__any(top * sl2 > m_run + kLazyMax)) {
-            const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32, 64)) * sl2);
-            const bool rise = m_new > m_run + kLazyMax;  // also the first finite maximum
-            const float al = rise ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
-            l_part *= al;
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-            for (int d = 0; d < DT; ++d) acc[d] *= al;
-            if constexpr (AFF) {
+          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, sc[kt][i]), sc[kt][i + 1]);
+        if (__any(top * sl2 > m_run + kLazyMax)) {
+          const float m_new = fmaxf(m_run, fmaxf(top, __shfl_xor(top, 32, 64)) * sl2);
+          const bool rise = m_new > m_run + kLazyMax;  // also the first finite maximum
+          const float al = rise ? __builtin_amdgcn_exp2f(m_run - m_new) : 1.f;
+          l_part *= al;
 #pragma unroll
-              for (int g = 0; g < G; ++g) pb[g] *= al;
-            }
-            if (rise) m_run = m_new;
-          }
-          constexpr int DG = DT / G;  // dim tiles of a quantization group
-          Op va[DT];
-          if constexpr (!AFF) {
-#pragma unroll
-            for (int d = 0; d < DT; ++d) va[d] = read_v(kt, 0, d);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-          // p <= 2^(kLazyMax + 6), times a value scale below 2: inside fp16, and small p stay clear of its sub-normals
-          const float m_sub = fmaxf(m_run, -3.0e38f) - 6.f;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], sl2, -m_sub));
-            l_part += sc[i];
-          }
-          // ---- O^T += V^T P^T, 16 keys at a time
+          for (int d = 0; d < DT; ++d) acc[d] *= al;
           if constexpr (AFF) {
-            const float *vsf = ksf + G * NT, *vbf = vsf + G * NT;
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int g = 0; g < G; ++g) {
-#pragma unroll
-                for (int d = 0; d < DG; ++d) va[d] = read_v(kt, j, g * DG + d);
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const f32x4 vs4 = *reinterpret_cast<const f32x4*>(vsf + g * NT + k0 + 16 * j + 8 * e + 4 * half);
-                  const f32x4 vb4 = *reinterpret_cast<const f32x4*>(vbf + g * NT + k0 + 16 * j + 8 * e + 4 * half);
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) {
-                    const float p = sc[8 * j + 4 * e + r];
-                    x[4 * e + r] = p * vs4[r];
-                    pb[g] = fmaf(p, vb4[r], pb[g]);
-                  }
-                }
-                Op pB[2];
-                split_p2(x, pB);
-#pragma unroll
-                for (int k = 0; k < 2; ++k)
-#pragma unroll
-                  for (int d = 0; d < DG; ++d) acc[g * DG + d] = mfma32(va[d], pB[k], acc[g * DG + d]);
-                __builtin_amdgcn_sched_barrier(0);  // (the scales' reads stay with their group)
-              }
-            if (kk + 1 < KT) {
-#pragma unroll
-              for (int i = 0; i < KA; ++i) ka[i] = read_k(kt - 1, i);
-            }
-          } else {
-            Op pB[2][2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = sc[8 * j + e];
-              if constexpr (FP8) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const f32x4 vs4 = *reinterpret_cast<const f32x4*>(ksf + NT + k0 + 16 * j + 8 * e + 4 * half);
-#pragma unroll
-                  for (int r = 0; r < 4; ++r) x[4 * e + r] *= vs4[r];
-                }
-              }
-              split_p2(x, pB[j]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            Op vb[DT];
-#pragma unroll
-            for (int d = 0; d < DT; ++d) vb[d] = read_v(kt, 1, d);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int d = 0; d < DT; ++d) acc[d] = mfma32(va[d], pB[0][k], acc[d]);
-            __builtin_amdgcn_sched_barrier(0);
-            if (kk + 1 < KT) {
-#pragma unroll
-              for (int i = 0; i < KA; ++i) ka[i] = read_k(kt - 1, i);
-              __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int d = 0; d < DT; ++d) acc[d] = mfma32(vb[d], pB[1][k], acc[d]);
+            for (int g = 0; g < GV; ++g) pb[g] *= al;
           }
+          if (rise) m_run = m_new;
+        }
+        // p <= 2^(kLazyMax + 6), times a value scale below 2: inside fp16, and small p stay clear of its sub-normals
+        const float m_sub = fmaxf(m_run, -3.0e38f) - 6.f;
+
+        // ---- O^T += V^T P^T in steps of 16 keys (and one group); a step's operands are made while the products of the step
+        // before it run (affine: right before its own, they have too many registers)
+        constexpr int AH = AFF ? 0 : 1;
+        constexpr int DG = DT / GV, US = KT * 2 * GV;  // dim tiles of a group, steps
+        Op va[1 + AH][DG], pB[1 + AH][2];
+        auto make = [&](const int u) {
+          const int kt = KT - 1 - u / (2 * GV), j = u / GV % 2, g = u % GV, k0 = (kw * KT + kt) * 32 + 16 * j + 4 * half;
+#pragma unroll
+          for (int d = 0; d < DG; ++d) va[u & AH][d] = read_v(kt, j, g * DG + d);
+          if (g == 0) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              sc[kt][8 * j + e] = __builtin_amdgcn_exp2f(fmaf(sc[kt][8 * j + e], sl2, -m_sub));
+              l_part += sc[kt][8 * j + e];
+            }
+          }
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = sc[kt][8 * j + e];
+          if constexpr (AFF || FP8) {
+            const float *vsf = ksf + (FP8 ? 1 : G + GV * dw + g) * NT + k0, *vbf = vsf + G * NT;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const f32x4 vs4 = *reinterpret_cast<const f32x4*>(vsf + 8 * e);
+              if constexpr (AFF) {
+                const f32x4 vb4 = *reinterpret_cast<const f32x4*>(vbf + 8 * e);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) pb[g] = fmaf(x[4 * e + r], vb4[r], pb[g]);
+              }
+#pragma unroll
+              for (int r = 0; r < 4; ++r) x[4 * e + r] *= vs4[r];
+            }
+          }
+          split_p2(x, pB[u & AH]);
+        };
+        if constexpr (AH) {
+          make(0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int u = 0; u < US; ++u) {
+          if constexpr (!AH) make(u);
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int d = 0; d < DG; ++d)
+              acc[u % GV * DG + d] = mfma32(va[u & AH][d], pB[u & AH][k], acc[u % GV * DG + d]);
+          if constexpr (AH) {
+            if (u + 1 < US) make(u + 1);
+#pragma unroll
+            for (int i = 0; i < 2 * DG; ++i) {
+              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
+              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+              __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);    // what the vector unit does meanwhile
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -966,10 +1035,10 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
     if constexpr (AFF) {  // codes entered as code * 2^-kCodeExp; the bias term joins its group's dims
       const float f = __uint_as_float((uint32_t)(127 + vexp + C::kCodeExp) << 23);
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
+      for (int g = 0; g < GV; ++g) {
         const float bias = pb[g] + __shfl_xor(pb[g], 32, 64);
 #pragma unroll
-        for (int d = g * DT / G; d < (g + 1) * DT / G; ++d) acc[d] = acc[d] * f + bias;
+        for (int d = g * DT / GV; d < (g + 1) * DT / GV; ++d) acc[d] = acc[d] * f + bias;
       }
     }
     if constexpr (FP8) {  // the codes entered as value * 2^-8
@@ -1011,11 +1080,12 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
     }
 
     const bool whole = b0 == 0 && b1 == nblk;
-    if (nwg > 0 && b0 == 0 && tid == 0) {
-      // who has the tile's last block, counting this range's as the first
-      const int g0 = (int)((long long)(w + 1) * all / nwg) - todo;  // the tile's first block in the launch
-      const int wl = whole ? w : (int)(((long long)(g0 + nblk) * nwg - 1) / all);
-      A.desc[1 + (size_t)kvh * A.tiles + t] = int4{sq.s, tile, whole ? 1 : wl - w + 1, 2 * w + (first_seg ? 0 : 1)};
+    if (nwg > 0 && b0 == 0) {
+      const int g0 = ranges.begin(w + 1) - todo - u0;  // the tile's first unit in the launch
+      if (!whole)
+        cut_tile = int4{sq.s, tile, kvh * kWideParts + ranges.owner(g0 + kWideBegin + nblk - 1) - w + 1,
+                        2 * w + (first_seg ? 0 : 1)};
+      if (by_tile && tid == 0) A.desc[1 + kvh * A.tiles + t] = cut_tile;
     }
     if (kw == 0) {
       if (whole) {
@@ -1027,7 +1097,7 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
           for (int j = 0; j < 4; ++j)
             bad |= masked_write<C, D>(a, sq, kvh, tok, head,
                                       f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, l,
-                                      inv, 32 * d + 8 * j + 4 * half);
+                                      inv, 32 * (dw * DT + d) + 8 * j + 4 * half);
         uint64_t again = __ballot(bad);
         again = (again | (again >> 32)) & 0xFFFFFFFFull;
         if (again) {
@@ -1035,101 +1105,109 @@ __global__ __launch_bounds__(256, (D == 256 || (C::kAffine && D == 128 && KW == 
           for (; again; again &= again - 1) {
             const int c = __builtin_ctzll(again);
             attend_masked<C, D>(a, mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c),
-                                lane);
+                                lane, dw * DT * 32, (dw + 1) * DT * 32);
           }
         }
       } else {
-        f32x4* st = reinterpret_cast<f32x4*>(A.part + (size_t)(2 * w + (first_seg ? 0 : 1)) * kWidePart<D, KW>) +
+        f32x4* st = reinterpret_cast<f32x4*>(A.part + (size_t)(2 * w + (first_seg ? 0 : 1)) * kWidePart<D, CW>) +
                     (size_t)cw * (D / 8 + 1) * 64 + lane;
         if (tok >= 0) {
 #pragma unroll
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              st[(4 * d + j) * 64] = f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
+              st[(4 * (dw * DT + d) + j) * 64] = f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]};
         }
-        st[(D / 8) * 64] = f32x4{m_run, l, 0.f, 0.f};
+        if (dw == 0) st[(D / 8) * 64] = f32x4{m_run, l, 0.f, 0.f};
       }
     }
-    if (nwg == 0) return;
-    todo -= b1 - b0;
-    if (todo <= 0) return;
     first_seg = false;
-    b0 = 0;
+    }
+    if (nwg == 0) return;
+    todo -= u1 - u0;
+    if (todo <= 0) break;
+    u0 = 0;
     if (++t == ntiles) {
       t = 0;
       ++kvh;
       sidx = 0;
     }
   }
+  if (!by_tile && tid == 0) A.desc[1 + w] = cut_tile;
 }
 
-// Joins the parts of cut tiles, in part order.  Grid (tiles * Hkv, column waves, D / 32): a workgroup has 32 columns and
-// 32 dims of one tile, a wave 8 of them, 8 parts in flight.
-template <class C, int D, int KW>
+// Joins the parts of cut tiles, in part order.  Grid (descriptors, column waves, a divisor of D / 32): a workgroup has 32
+// columns of one tile and goes over its share of the dims 32 at a time, a wave 8 of them, 8 parts in flight.
+template <class C, int D, int CW>
 __global__ __launch_bounds__(256) void masked_merge(MaskedArgs A) {
   const DecodeArgs& a = A.d;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), cw = blockIdx.y;
-  const int kvh = blockIdx.x / A.tiles, t = blockIdx.x % A.tiles;
-  if (t >= A.desc[0].x) return;
-  const int4 de = A.desc[1 + blockIdx.x];
-  const int np = de.z;
-  if (np <= 1) return;
-  const int c32 = lane & 31, half = lane >> 5, vec = 4 * blockIdx.z + wv;
+  const bool by_tile = a.Hkv * A.tiles <= A.wgs;
+  // (descriptors in the order of the workgroups that wrote the parts, XCD by XCD)
+  const int n = gridDim.x, id = n % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (n / 8) + (int)blockIdx.x / 8;
+  const int4 de = A.desc[1 + id];
+  if ((by_tile ? id % A.tiles : id) >= A.desc[0].x) return;
+  const int np = de.z % kWideParts, kvh = de.z / kWideParts;
+  if (np == 0) return;
+  const int c32 = lane & 31, half = lane >> 5;
   const f32x4* base = reinterpret_cast<const f32x4*>(A.part) + (size_t)cw * (D / 8 + 1) * 64 + lane;
   // the first part's slot, then the first slots of the workgroups that follow
   const int slot0 = de.w, next0 = (de.w | 1) + 1;
-  auto slot = [&](const int q) { return (size_t)(q == 0 ? slot0 : next0 + 2 * (q - 1)) * (kWidePart<D, KW> / 4); };
+  auto slot = [&](const int q) { return (size_t)(q == 0 ? slot0 : next0 + 2 * (q - 1)) * (kWidePart<D, CW> / 4); };
   constexpr int U = 8;
   const MaskedSeq sq = masked_seq(A, de.x);
-  float m = -INFINITY, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int q0 = 0; q0 < np; q0 += U) {
-    f32x4 x[U];
-    f32x2 ml[U];
-#pragma unroll
-    for (int k = 0; k < U; ++k) {  // (past the last part: that one again, of no weight)
-      const f32x4* st = base + slot(min(q0 + k, np - 1));
-      ml[k] = *reinterpret_cast<const f32x2*>(st + (D / 8) * 64);
-      x[k] = st[vec * 64];  // (a column that is none holds anything: its lanes write nothing)
-    }
-    float top = m;
-#pragma unroll
-    for (int k = 0; k < U; ++k) top = fmaxf(top, ml[k][0]);
-    // (a part without a live key has m = -inf and zeros, one of NaN scores only a sum that is NaN)
-    auto weight = [&](const float m1, const float l1) {
-      return m1 == -INFINITY ? (l1 == 0.f ? 0.f : l1) : __builtin_amdgcn_exp2f(m1 - top);
-    };
-    const float f0 = weight(m, l);
-    l *= f0;
-    o *= f0;
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (q0 + k < np) {
-        const float f = weight(ml[k][0], ml[k][1]);
-        l = fmaf(ml[k][1], f, l);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = fmaf(x[k][r], f, o[r]);
-      }
-    }
-    m = top;
-  }
   int tok, head;
   masked_column(A, sq, de.y, cw * 32 + c32, a.Hq / a.Hkv, tok, head);
-  const bool bad = masked_write<C, D>(a, sq, kvh, tok, head, o, l, l > 0.f ? 1.f / l : 0.f,
-                                      32 * (vec / 4) + 8 * (vec % 4) + 4 * half);
-  // rows that are not finite here: these 32 dims again in fp32
   __shared__ unsigned int again[4];
-  const uint64_t b = __ballot(bad);
-  if (lane == 0) again[wv] = (unsigned int)(b | (b >> 32));
-  __builtin_amdgcn_s_waitcnt(0);  // (the first results are out before the second)
-  __syncthreads();
-  unsigned int all = __builtin_amdgcn_readfirstlane(again[0] | again[1] | again[2] | again[3]);
-  for (; all; all &= all - 1) {
-    const int c = __builtin_ctz(all);
-    if ((c & 3) == wv)
-      attend_masked<C, D>(a, A.mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c),
-                          lane, 32 * blockIdx.z, 32 * blockIdx.z + 32);
+  for (int z = blockIdx.z; z < D / 32; z += gridDim.z) {
+    const int vec = 4 * z + wv;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int q0 = 0; q0 < np; q0 += U) {
+      f32x4 x[U];
+      f32x2 ml[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {  // (past the last part: that one again, of no weight)
+        const f32x4* st = base + slot(min(q0 + k, np - 1));
+        ml[k] = *reinterpret_cast<const f32x2*>(st + (D / 8) * 64);
+        x[k] = st[vec * 64];  // (a column that is none holds anything: its lanes write nothing)
+      }
+      float top = m;
+#pragma unroll
+      for (int k = 0; k < U; ++k) top = fmaxf(top, ml[k][0]);
+      // (a part without a live key has m = -inf and zeros, one of NaN scores only a sum that is NaN)
+      auto weight = [&](const float m1, const float l1) {
+        return m1 == -INFINITY ? (l1 == 0.f ? 0.f : l1) : __builtin_amdgcn_exp2f(m1 - top);
+      };
+      const float f0 = weight(m, l);
+      l *= f0;
+      o *= f0;
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (q0 + k < np) {
+          const float f = weight(ml[k][0], ml[k][1]);
+          l = fmaf(ml[k][1], f, l);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[r] = fmaf(x[k][r], f, o[r]);
+        }
+      }
+      m = top;
+    }
+    const bool bad = masked_write<C, D>(a, sq, kvh, tok, head, o, l, l > 0.f ? 1.f / l : 0.f,
+                                        32 * (vec / 4) + 8 * (vec % 4) + 4 * half);
+    // rows that are not finite here: these 32 dims again in fp32
+    const uint64_t b = __ballot(bad);
+    if (lane == 0) again[wv] = (unsigned int)(b | (b >> 32));
+    __builtin_amdgcn_s_waitcnt(0);  // (the first results are out before the second)
+    __syncthreads();
+    unsigned int all = __builtin_amdgcn_readfirstlane(again[0] | again[1] | again[2] | again[3]);
+    for (; all; all &= all - 1) {
+      const int c = __builtin_ctz(all);
+      if ((c & 3) == wv)
+        attend_masked<C, D>(a, A.mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c),
+                            lane, 32 * z, 32 * z + 32);
+    }
+    __syncthreads();  // (again is free)
   }
 }
 
