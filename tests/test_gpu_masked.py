@@ -306,3 +306,28 @@ def test_captured_calls(cuda):
         check(a, got, expected(dict(a, kvl=lens), 0, 0, pa))
         assert np.array_equal(got, eager.double().cpu().numpy())
         check(w, graphs[1][1].double().cpu().numpy(), expected(w, 2000, 4))
+
+
+@pytest.mark.parametrize("count", [300, 1100])
+@pytest.mark.parametrize("kind", ["bf16", "fp8", "q4"])
+def test_many_sequences(cuda, kind, count):
+    """More sequences than the kernel keeps in LDS, and more than it takes (the general kernel's): none to three tokens."""
+    print(f"[{count} sequences {kind}]", flush=True)
+    rng = np.random.default_rng(count)
+    qlens = [int(x) for x in rng.integers(0, 4, count)]
+    kvl = [q + int(x) for q, x in zip(qlens, rng.integers(0, 90, count))]
+    b = batch(kind, qlens, kvl, 8, 2, 64, 16, seed=count, gs=64)
+    for window, sinks in ((17, 3), (40, 20)):
+        check(b, run(b, cuda, window, sinks), expected(b, window, sinks))
+    p = trees(b, count)
+    check(b, run(b, cuda, 0, 0, p), expected(b, 0, 0, p))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_more_tiles_than_workgroups(cuda, kind):
+    """Long prompts and trees of many heads: a workgroup to a tile, none of them cut."""
+    print(f"[many tiles {kind}]", flush=True)
+    b = batch(kind, [700, 33, 700, 700], [700, 400, 731, 705], 64, 8, 128, 32, seed=3, gs=64)
+    check(b, run(b, cuda, 24, 2), expected(b, 24, 2))
+    p = trees(b, 7)
+    check(b, run(b, cuda, 30, 5, p), expected(b, 30, 5, p))
