@@ -85,11 +85,12 @@ struct MaskedArgs {
 };
 
 // What beginning a tile costs (pages, queries, first block; a part written), in blocks: 6 to 9 us against 2 to 3 us a block.
-// Ranges are equal with it: without, those of short tiles ended last.
+// Ranges are equal with it, else those of short tiles end last (32 trees of 16 nodes on 4-bit pages: 92 us against 99, three
+// prompt chunks with 256-wide heads 73 against 76).  A range may be one block: a tree of 25 nodes over 1531 keys takes 19.4
+// us against 21.5 with two at least.
 constexpr int kWideBegin = 3;
-// Fewest blocks of a workgroup's range; and how many blocks longer than an equal share the longest tile may be before
-// tiles are cut, where there is a workgroup for each (parts go to memory and back: 64 KiB each way, and a launch).
-constexpr int kWideRangeBlocks = 2;
+// How many blocks longer than an equal share the longest tile may be before tiles are cut, where there is a workgroup for
+// each (parts go to memory and back: 64 KiB each way, and a launch).
 constexpr int kWideCutBlocks = 6;
 constexpr int kWideParts = 1024;   // more than a tile's parts
 constexpr int kWideTreeLds = 512;  // nodes of a tree whose parents are kept in LDS
@@ -470,7 +471,7 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
 #pragma unroll
     for (int i = 0; i < NW; ++i) most = max(most, red[8 + i]);
     const int all = per * a.Hkv;  // (the host keeps it below 2^31)
-    nwg = min(A.wgs, max(1, all / kWideRangeBlocks));
+    nwg = min(A.wgs, max(1, all));
     if (nwg >= 8) nwg &= ~7;
     const int nt = ntiles * a.Hkv;
     if (nt <= A.wgs && most <= all / nwg + kWideCutBlocks) {  // a tile to a workgroup
