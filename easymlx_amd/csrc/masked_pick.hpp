@@ -11,10 +11,12 @@ void launch_masked_kernels(const MaskedArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((masked_wide<C, D, KW, CW>), dim3((unsigned)(a.wgs > 0 ? a.wgs : tiles)),
                      dim3((WideCfg<C, D, KW, CW>::TH)), 0, st, a);
   if (a.wgs > 0) {
-    const int n = tiles < a.wgs ? tiles : a.wgs;
-    int z = D / 32;  // (workgroups without work cost 2 ns each)
-    while (z > 1 && n * CW * z > 2048) z /= 2;
-    hipLaunchKernelGGL((masked_merge<C, D, CW>), dim3((unsigned)n, CW, z), dim3(256), 0, st, a);
+    const unsigned n = tiles < a.wgs ? tiles : a.wgs;
+    if (n * CW <= 128)
+      hipLaunchKernelGGL((masked_merge<C, D, CW, 1>), dim3(n, CW, D / 32), dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((masked_merge<C, D, CW, 4>), dim3(n, CW, D > 128 ? D / 128 : 1), dim3(D < 128 ? 2 * D : 256), 0,
+                         st, a);
   }
 }
 

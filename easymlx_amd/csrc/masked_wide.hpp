@@ -39,6 +39,8 @@
 // pages the vector unit (codes to values, scales, softmax: 480 instructions a block and wave).
 #pragma once
 
+#include <type_traits>
+
 #include "masked_launch.hpp"
 #include "prefill_mfma.hpp"
 
@@ -1137,12 +1139,15 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
   if (!by_tile && tid == 0) A.desc[1 + w] = cut_tile;
 }
 
-// Joins the parts of cut tiles, in part order.  Grid (descriptors, column waves, a divisor of D / 32): a workgroup has 32
-// columns of one tile and goes over its share of the dims 32 at a time, a wave 8 of them, 8 parts in flight.
-template <class C, int D, int CW>
-__global__ __launch_bounds__(256) void masked_merge(MaskedArgs A) {
+// Joins the parts of cut tiles, in part order.  Grid (descriptors, column waves, dims / 32 NV): a wave has 32 columns and 8 NV
+// dims of one tile, its workgroup 32 NV.  Bound by the parts' way to memory and back (256 columns: 131 KB each): NV = 4, 192
+// tiles in two or three parts 17 us (NV = 1 with eight loads a round however few the parts: 34), but NV = 1 where
+// descriptors are few and their parts many: a tree of 25 nodes in 24 parts 5.4 us against 7.8.
+template <class C, int D, int CW, int NV>
+__global__ __launch_bounds__(NV * 32 > D ? 8 * D / NV : 256) void masked_merge(MaskedArgs A) {
   const DecodeArgs& a = A.d;
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), cw = blockIdx.y;
+  const int lane = threadIdx.x & 63, cw = blockIdx.y;
+  const int v0 = (blockIdx.z * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * NV;  // dims 8 v0 ..
   const bool by_tile = a.Hkv * A.tiles <= A.wgs;
   // (descriptors in the order of the workgroups that wrote the parts, XCD by XCD)
   const int n = gridDim.x, id = n % 8 ? (int)blockIdx.x : (int)(blockIdx.x % 8) * (n / 8) + (int)blockIdx.x / 8;
@@ -1155,23 +1160,26 @@ __global__ __launch_bounds__(256) void masked_merge(MaskedArgs A) {
   // the first part's slot, then the first slots of the workgroups that follow
   const int slot0 = de.w, next0 = (de.w | 1) + 1;
   auto slot = [&](const int q) { return (size_t)(q == 0 ? slot0 : next0 + 2 * (q - 1)) * (kWidePart<D, CW> / 4); };
-  constexpr int U = 8;
   const MaskedSeq sq = masked_seq(A, de.x);
   int tok, head;
   masked_column(A, sq, de.y, cw * 32 + c32, a.Hq / a.Hkv, tok, head);
-  __shared__ unsigned int again[4];
-  for (int z = blockIdx.z; z < D / 32; z += gridDim.z) {
-    const int vec = 4 * z + wv;
-    float m = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if (!__any(tok >= 0)) return;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[NV] = {};
+  auto join = [&](auto parts) {
+    constexpr int U = decltype(parts)::value;
     for (int q0 = 0; q0 < np; q0 += U) {
-      f32x4 x[U];
+      f32x4 x[U][NV];
       f32x2 ml[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) {  // (past the last part: that one again, of no weight)
-        const f32x4* st = base + slot(min(q0 + k, np - 1));
-        ml[k] = *reinterpret_cast<const f32x2*>(st + (D / 8) * 64);
-        x[k] = st[vec * 64];  // (a column that is none holds anything: its lanes write nothing)
+      for (int k = 0; k < U; ++k) {
+        ml[k] = f32x2{-INFINITY, 0.f};
+        if (q0 + k < np) {
+          const f32x4* st = base + slot(q0 + k);
+          ml[k] = *reinterpret_cast<const f32x2*>(st + (D / 8) * 64);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) x[k][j] = st[(v0 + j) * 64];  // (a column that is none holds anything)
+        }
       }
       float top = m;
 #pragma unroll
@@ -1182,33 +1190,37 @@ __global__ __launch_bounds__(256) void masked_merge(MaskedArgs A) {
       };
       const float f0 = weight(m, l);
       l *= f0;
-      o *= f0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) o[j] *= f0;
 #pragma unroll
       for (int k = 0; k < U; ++k) {
         if (q0 + k < np) {
           const float f = weight(ml[k][0], ml[k][1]);
           l = fmaf(ml[k][1], f, l);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) o[r] = fmaf(x[k][r], f, o[r]);
+          for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[j][r] = fmaf(x[k][j][r], f, o[j][r]);
         }
       }
       m = top;
     }
-    const bool bad = masked_write<C, D>(a, sq, kvh, tok, head, o, l, l > 0.f ? 1.f / l : 0.f,
-                                        32 * (vec / 4) + 8 * (vec % 4) + 4 * half);
-    // rows that are not finite here: these 32 dims again in fp32
-    const uint64_t b = __ballot(bad);
-    if (lane == 0) again[wv] = (unsigned int)(b | (b >> 32));
-    __builtin_amdgcn_s_waitcnt(0);  // (the first results are out before the second)
-    __syncthreads();
-    unsigned int all = __builtin_amdgcn_readfirstlane(again[0] | again[1] | again[2] | again[3]);
-    for (; all; all &= all - 1) {
-      const int c = __builtin_ctz(all);
-      if ((c & 3) == wv)
-        attend_masked<C, D>(a, A.mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c),
-                            lane, 32 * z, 32 * z + 32);
+  };
+  np <= 3 ? join(std::integral_constant<int, 3>{}) : join(std::integral_constant<int, 8>{});
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) bad |= masked_write<C, D>(a, sq, kvh, tok, head, o[j], l, inv, 8 * (v0 + j) + 4 * half);
+  // rows that are not finite here: these dims again in fp32
+  uint64_t again = __ballot(bad);
+  again = (again | (again >> 32)) & 0xFFFFFFFFull;
+  if (again) {
+    __builtin_amdgcn_s_waitcnt(0);  // (the rows' first results are out before their second)
+    for (; again; again &= again - 1) {
+      const int c = __builtin_ctzll(again);
+      attend_masked<C, D>(a, A.mask, sq, kvh, __builtin_amdgcn_readlane(tok, c), __builtin_amdgcn_readlane(head, c), lane,
+                          8 * v0, 8 * (v0 + NV));
     }
-    __syncthreads();  // (again is free)
   }
 }
 
