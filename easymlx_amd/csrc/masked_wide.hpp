@@ -146,14 +146,17 @@ __device__ __forceinline__ constexpr int va_turn(const int dim, const int c) {
   return c ^ (NT == 64 ? (dim >> 1) & 7 : (dim >> 2) & 3);
 }
 
-// 16 bytes from `src` (each lane its own) to LDS byte `dst` + 16 lane, with no register between.  Nothing waits for it but
-// dma_wait: the compiler's own waits count only loads that it knows, which come back in order with these.  (By the
+// 16 bytes from src + off (each lane its own) to LDS byte `dst` + 16 lane, with no register between.  Nothing waits for it
+// but dma_wait: the compiler's own waits count only loads that it knows, which come back in order with these.  (By the
 // compiler's builtin every transposing LDS read that follows waits for it, in the block before the one it loads.)
-__device__ __forceinline__ void dma16(const void* src, const uint32_t dst) {
+__device__ __forceinline__ void dma16(const char* src, const uint32_t off, const uint32_t dst) {
+  const uint64_t a = reinterpret_cast<uint64_t>(src);
+  const uint64_t base = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) |
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(m0)
-               : "v"(src), "s"(__builtin_amdgcn_readfirstlane(dst))
+               : "v"(off), "s"(base), "s"(dst)
                : "memory");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
@@ -238,6 +241,8 @@ __device__ __forceinline__ int wg_scan(const int mine, int* red, int& total) {
     base += w < wv ? red[w] : 0;
     total += red[w];
   }
+  // (what comes from LDS counts as each lane's own: every address and bound reckoned from it was, in vector registers)
+  total = __builtin_amdgcn_readfirstlane(total);
   return base + x - mine;
 }
 
@@ -472,6 +477,7 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     const int before = wg_scan<NW>(mine, red, per);
 #pragma unroll
     for (int i = 0; i < NW; ++i) most = max(most, red[8 + i]);
+    most = __builtin_amdgcn_readfirstlane(most);
     const int all = per * a.Hkv;  // (the host keeps it below 2^31)
     nwg = min(A.wgs, max(1, all));
     if (nwg >= 8) nwg &= ~7;
@@ -491,7 +497,7 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     ranges = WideRanges(all, nwg);
     const int at = ranges.begin(w);
     todo = ranges.begin(w + 1) - at;
-    kvh = at / per;
+    kvh = __builtin_amdgcn_readfirstlane(at / per);
     const int r = at - kvh * per;
     if (r >= before && r < before + mine) {  // one thread's tiles hold it
       int x = before, i = 0, s = wide_seq_of(tcum, S, t0);
@@ -524,6 +530,13 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
   const size_t rowb = (size_t)a.Hkv * D * sizeof(typename C::ET);  // token-major
   typedef __attribute__((address_space(3))) unsigned char* lptr;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lptr)lds;
+  uint32_t dma_k = 0, dma_v = 0;  // DMA: a lane's byte among the rows that its wave loads, of K and of V
+  if constexpr (DMA) {
+    static_assert(TH / P::PR % 16 == 0, "a thread's next rows are turned as its first");
+    const int r = tid / P::PR, c = tid % P::PR;
+    dma_k = lane / P::PR * (uint32_t)rowb + 16 * k_turn<D>(r, c);
+    dma_v = lane / P::PR * (uint32_t)rowb + 16 * v_turn<D>(r, c);
+  }
 
   int sidx = wide_seq_of(tcum, S, t);
   for (;;) {
@@ -564,9 +577,26 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     float psk = 0.f, psv = 0.f;            // FP8: page scales of key `lane` of that block
     auto load_block = [&](const int st, const int blk, const int buf) {
       const unsigned tid = anew(threadIdx.x), lane = tid & 63;
-      const int pos = min(pos_of_block(st) + (lane & (NT - 1)), k_hi);
       const bool ok = (unsigned)blk < (unsigned)a.nb;
       okn = __ballot(ok);
+      if constexpr (DMA) {
+        // A wave's 64 pieces, DR rows of one page (its tokens are a multiple of 8), stand in a row in the image: each lane
+        // takes the chunk that belongs there.  What is the wave's is reckoned by the scalar unit
+        constexpr int DR = 64 / P::PR;
+#pragma unroll
+        for (int n = 0; n < P::NP; ++n) {
+          const int r0 = (wv + n * (TH / 64)) * DR, s = min(pos_of_block(st) + r0, k_hi);
+          const int id = __builtin_amdgcn_readlane(blk, r0), b = (unsigned)id < (unsigned)a.nb ? id : 0;
+          const size_t o = (size_t)(b * a.bs + s - page_of(s, A.inv_bs) * a.bs) * rowb;
+          const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + oBuf + buf * BUF + (wv + n * (TH / 64)) * 1024);
+          uint32_t back = 0;  // rows past the tile's last key repeat it
+          if (s + DR - 1 > k_hi) back = (uint32_t)max((int)(lane / P::PR) - (k_hi - s), 0) * (uint32_t)rowb;
+          dma16(kbase + o, dma_k - back, dst);
+          dma16(vbase + o, dma_v - back, dst + oV);
+        }
+        return;
+      }
+      const int pos = min(pos_of_block(st) + (lane & (NT - 1)), k_hi);
       const int b = ok ? blk : 0;
       const int off = pos - page_of(pos, A.inv_bs) * a.bs;
       if constexpr (AFF) {
@@ -603,14 +633,8 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
         for (int n = 0; n < P::NP; ++n) {
           const int r = tid / P::PR + n * (TH / P::PR), c = (int)(tid % P::PR);
           const size_t o = (size_t)__shfl(row, r, 64) * rowb;
-          if constexpr (DMA) {  // a wave's 64 pieces stand in a row in the image: each lane takes the chunk that belongs there
-            const uint32_t dst = lds0 + oBuf + buf * BUF + (wv + n * (TH / 64)) * 1024;
-            dma16(kbase + o + 16 * k_turn<D>(r, c), dst);
-            dma16(vbase + o + 16 * v_turn<D>(r, c), dst + oV);
-          } else {
-            rk[n] = *reinterpret_cast<const u32x4*>(kbase + o + 16 * c);
-            rv[n] = *reinterpret_cast<const u32x4*>(vbase + o + 16 * c);
-          }
+          rk[n] = *reinterpret_cast<const u32x4*>(kbase + o + 16 * c);
+          rv[n] = *reinterpret_cast<const u32x4*>(vbase + o + 16 * c);
         }
       }
     };
