@@ -148,13 +148,14 @@ __device__ __forceinline__ constexpr int va_turn(const int dim, const int c) {
 
 // 16 bytes from src + off (each lane its own) to LDS byte `dst` + 16 lane, with no register between.  Nothing waits for it
 // but dma_wait: the compiler's own waits count only loads that it knows, which come back in order with these.  (By the
-// compiler's builtin every transposing LDS read that follows waits for it, in the block before the one it loads.)
+// compiler's builtin every transposing LDS read that follows waits for it, in the block before the one it loads.  A write
+// of m0 needs one wait state before a load that goes by it.)
 __device__ __forceinline__ void dma16(const char* src, const uint32_t off, const uint32_t dst) {
   const uint64_t a = reinterpret_cast<uint64_t>(src);
   const uint64_t base = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32)) << 32) |
                         (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
   uint32_t m0;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b32 m0, %0"
                : "=&s"(m0)
                : "v"(off), "s"(base), "s"(dst)
                : "memory");
@@ -428,7 +429,6 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
   constexpr int oBuf = 0, KB = NT * D * 2, oV = KB, oSc = oV + P::VB;
   constexpr int BUF = (oSc + (DMA ? 0 : P::SCB + 16) + 511) & ~511;
   static_assert(KB % 512 == 0 && P::VB % 512 == 0, "the images' chunks are flipped by address bits");
-  static_assert(!DMA || 2 * BUF <= 65536, "where dma16 may write: its LDS address has 16 bits");
   constexpr int MEET = KW > 1 ? CW * (4 * DT + 1) * 64 * 16 : 0;
   constexpr int oTc = 2 * BUF > MEET ? 2 * BUF : MEET, oSeq = lds_next(oTc, 4 * (kWideSeqs + 1));
   constexpr int oPar = lds_next(oSeq, 12 * kWideSeqLds), oRed = lds_next(oPar, 4 * kWideTreeLds);
@@ -570,7 +570,7 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     auto page_id = [&](const int st) {
       return bt[page_of(min(pos_of_block(st) + (lane & (NT - 1)), k_hi), A.inv_bs)];
     };
-    u32x4 rk[P::NP], rv[AFF ? 1 : P::NP];  // the next block's pieces (DMA: none)
+    u32x4 rk[P::NP], rv[AFF ? 1 : P::NP];  // the next block's pieces (DMA: not used)
     u32x2 ru[AFF ? 16 : 1];                // affine: its V units
     u32x4 rs;                              // affine, wave 0: scale piece `lane`
     uint64_t okn = 0;                      // keys of that block on a valid page
@@ -996,14 +996,13 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
         const float m_sub = fmaxf(m_run, -3.0e38f) - 6.f;
 
         // ---- O^T += V^T P^T in steps of 16 keys (and one group); a step's operands are made while the products of the step
-        // before it run (affine: right before its own, they have too many registers)
-        constexpr int AH = AFF ? 0 : 1;
+        // before it run
         constexpr int DG = DT / GV, US = KT * 2 * GV;  // dim tiles of a group, steps
-        Op va[1 + AH][DG], pB[1 + AH][2];
+        Op va[2][DG], pB[2][2];
         auto make = [&](const int u) {
           const int kt = KT - 1 - u / (2 * GV), j = u / GV % 2, g = u % GV, k0 = (kw * KT + kt) * 32 + 16 * j + 4 * half;
 #pragma unroll
-          for (int d = 0; d < DG; ++d) va[u & AH][d] = read_v(kt, j, g * DG + d);
+          for (int d = 0; d < DG; ++d) va[u & 1][d] = read_v(kt, j, g * DG + d);
           if (g == 0) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -1028,32 +1027,26 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
               for (int r = 0; r < 4; ++r) x[4 * e + r] *= vs4[r];
             }
           }
-          split_p2(x, pB[u & AH]);
+          split_p2(x, pB[u & 1]);
         };
-        if constexpr (AH) {
-          make(0);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        make(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int u = 0; u < US; ++u) {
-          if constexpr (!AH) make(u);
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int d = 0; d < DG; ++d)
-              acc[u % GV * DG + d] = mfma32(va[u & AH][d], pB[u & AH][k], acc[u % GV * DG + d]);
-          if constexpr (AH) {
-            if (u + 1 < US) make(u + 1);
+              acc[u % GV * DG + d] = mfma32(va[u & 1][d], pB[u & 1][k], acc[u % GV * DG + d]);
+          if (u + 1 < US) make(u + 1);
 #pragma unroll
-            for (int i = 0; i < 2 * DG; ++i) {
-              __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
-              __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
-              __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);    // what the vector unit does meanwhile
-            }
+          for (int i = 0; i < 2 * DG; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);    // a product
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+            __builtin_amdgcn_sched_group_barrier(0x2, 8, 0);    // what the vector unit does meanwhile
           }
           __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
       }
       if (st + 1 < st_hi) store_block(st + 1, buf ^ 1);
       __syncthreads();
