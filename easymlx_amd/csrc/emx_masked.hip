@@ -84,7 +84,7 @@ int check(const void* queries, int num_tokens, int num_q_heads, int head_dim, in
 template <typename QT, typename KV>
 int generic(const Call& c, const KV& kv) {
   const dim3 grid((unsigned)c.g.T, (unsigned)c.g.Hkv, (unsigned)((c.g.Hq / c.g.Hkv + 15) / 16));
-  hipLaunchKernelGGL((masked_generic<QT, KV>), grid, dim3(64), 0, c.st, c.g, c.mask, kv);
+  hipLaunchKernelGGL((masked_generic<QT, KV>), grid, dim3(64 * kGenericWaves), 0, c.st, c.g, c.mask, kv);
   return entry_check_launch("masked_generic");
 }
 

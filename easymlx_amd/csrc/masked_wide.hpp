@@ -453,7 +453,8 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
   // its blocks
   wide_tiles<NW>(A, tcum, seqs, red);
   if (row_lo > 0 || row_hi < A.T) zero_other_rows<QT>(a, A.T, D, blockIdx.x, gridDim.x);
-  const int ntiles = __builtin_amdgcn_readfirstlane(tcum[S]);
+  // (no more than the launch has room for, whatever query_start_loc holds)
+  const int ntiles = min(__builtin_amdgcn_readfirstlane(tcum[S]), A.tiles);
   int kvh, t, u0, todo, w = 0, nwg = 0;  // kv head, tile, unit within it, units left; nwg 0: no tile is cut
   WideRanges ranges(0, 1);
   if (A.wgs == 0) {

@@ -505,7 +505,7 @@ int emx_paged_attention_fp8(const void* queries, int num_tokens, int num_q_heads
  * on the order in which workgroups run.
  * fp16 / bf16 (queries' type) over unquantized caches, fp16 over FP8 and affine pages with
  * head_dim 64, 128 or 256, pages of a multiple of 8 tokens and 16-byte aligned tensors run on
- * the matrix units; other shapes, and fp32, on one wave per (token, kv head).
+ * the matrix units; other shapes, and fp32, on a workgroup per (token, kv head).
  * No counterpart in the reference.
  */
 int emx_masked_attention_affine(const void* queries, int num_tokens, int num_q_heads, int head_dim,
