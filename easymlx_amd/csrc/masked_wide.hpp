@@ -8,7 +8,7 @@
 //
 // in one pass over the keys with the running reference m_i.
 //
-// Work: a tile is the 32 CW query columns (token, head), head fastest, of COLS / HG tokens of one
+// Work: a tile is the 32 CW query columns (token, head), head fastest, of 32 CW / HG tokens of one
 // sequence and kv head; its keys go in blocks of NT positions, from the last backwards and then the
 // sinks' blocks: those between the sinks and the earliest window are not read.  From the last
 // backwards because a drafted node's ancestors then come in the order of its walk to the root: each
@@ -25,7 +25,7 @@
 // trees of 48 to 64 nodes with 64 / 8 heads and up to 32768 keys); FP8 (dec(code) * 2^-8, exact) and
 // affine codes (exact sub-normals) through registers.  A wave has 32 columns (KW = 2: and half of the
 // block's keys; D = 256: and half of the dims, the two halves of its scores meeting in LDS: a wave's
-// state then fits 256 registers, 83 -> 66 us over three prompt chunks on 8-bit pages), on v_mfma
+// state then fits 256 registers, 87 -> 77 us over three prompt chunks on 8-bit pages), on v_mfma
 // 32x32x16:
 //   S^T : A = K rows, B = queries; a lane ends with half of its tile's scores of ONE column, so that
 //         maximum, reference and sum are its own, and lanes meet only where a score passes the
@@ -35,8 +35,9 @@
 //         16, which puts an output off by at most 2^-17 of the largest value it averages: one part would
 //         add an error as large as the output's own rounding).
 // Bound: matrix instructions, 1.5 times the formula's for the second part, at the 1.27 PFLOP/s that a
-// large bf16 product reaches (those 12 trees: 543 us of the 745; without the loads 620); over affine
-// pages the vector unit (codes to values, scales, softmax: 480 instructions a block and wave).
+// large bf16 product reaches (those 12 trees, 461 GFLOP and 1.04 GB: 543 us of the 740; the matrix units
+// are busy in half of the cycles); over affine pages the vector unit and the chain of a block (codes to
+// values, scores, softmax: 20 vector instructions to a product).
 #pragma once
 
 #include <type_traits>
@@ -492,29 +493,29 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
       u0 = 0;
       todo = 0x7FFFFFFF;
     } else {
-    if ((int)blockIdx.x >= nwg) return;
-    // workgroups of one XCD (blockIdx mod 8) take neighbouring ranges: tiles of one sequence and kv head share its L2
-    w = nwg >= 8 ? (int)(blockIdx.x % 8) * (nwg / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
-    ranges = WideRanges(all, nwg);
-    const int at = ranges.begin(w);
-    todo = ranges.begin(w + 1) - at;
-    kvh = __builtin_amdgcn_readfirstlane(at / per);
-    const int r = at - kvh * per;
-    if (r >= before && r < before + mine) {  // one thread's tiles hold it
-      int x = before, i = 0, s = wide_seq_of(tcum, S, t0);
-      for (;; ++i) {
-        while (tcum[s + 1] <= t0 + i) ++s;
-        const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]) + kWideBegin;
-        if (r < x + n) break;
-        x += n;
+      if ((int)blockIdx.x >= nwg) return;
+      // workgroups of one XCD (blockIdx mod 8) take neighbouring ranges: tiles of one sequence and kv head share its L2
+      w = nwg >= 8 ? (int)(blockIdx.x % 8) * (nwg / 8) + (int)blockIdx.x / 8 : (int)blockIdx.x;
+      ranges = WideRanges(all, nwg);
+      const int at = ranges.begin(w);
+      todo = ranges.begin(w + 1) - at;
+      kvh = __builtin_amdgcn_readfirstlane(at / per);
+      const int r = at - kvh * per;
+      if (r >= before && r < before + mine) {  // one thread's tiles hold it
+        int x = before, i = 0, s = wide_seq_of(tcum, S, t0);
+        for (;; ++i) {
+          while (tcum[s + 1] <= t0 + i) ++s;
+          const int n = masked_blocks<NT>(A, wide_seq(A, seqs, s), t0 + i - tcum[s]) + kWideBegin;
+          if (r < x + n) break;
+          x += n;
+        }
+        red[16] = t0 + i;
+        red[17] = r - x;
       }
-      red[16] = t0 + i;
-      red[17] = r - x;
-    }
-    if (blockIdx.x == 0 && tid == 0) A.desc[0] = int4{by_tile ? ntiles : nwg, 0, 0, 0};
-    __syncthreads();
-    t = __builtin_amdgcn_readfirstlane(red[16]);
-    u0 = __builtin_amdgcn_readfirstlane(red[17]);
+      if (blockIdx.x == 0 && tid == 0) A.desc[0] = int4{by_tile ? ntiles : nwg, 0, 0, 0};
+      __syncthreads();
+      t = __builtin_amdgcn_readfirstlane(red[16]);
+      u0 = __builtin_amdgcn_readfirstlane(red[17]);
     }
   }
 
@@ -540,6 +541,16 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
   }
 
   int sidx = wide_seq_of(tcum, S, t);
+  auto next = [&](const int done) {  // on to the range's next tile, if there is one
+    todo -= done;
+    u0 = 0;
+    if (++t == ntiles) {
+      t = 0;
+      ++kvh;
+      sidx = 0;
+    }
+    return todo > 0;
+  };
   for (;;) {
     // ---- a segment: blocks [b0, b1) of tile t
     while (tcum[sidx + 1] <= t) ++sidx;
@@ -553,7 +564,10 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     const MaskedSpan span = masked_span<NT>(mask, past, tok_lo, tok_hi);
     const int nblk = max(1, span.n), u1 = min(nblk + kWideBegin, u0 + min(todo, nblk + kWideBegin - u0));
     const int b0 = max(0, u0 - kWideBegin), b1 = max(0, u1 - kWideBegin);
-    if (b0 < b1) {
+    if (b0 == b1) {  // a range that ends in what it costs to begin this tile leaves it to the next
+      if (!next(u1 - u0)) break;
+      continue;
+    }
     const int st_lo = b0, st_hi = min(b1, span.n);  // (an empty tile has a block of nothing)
     const int k_hi = max(past + tok_hi, 0);
     const int32_t* par = mask.parents ? mask.parents + q0 : nullptr;
@@ -1143,16 +1157,8 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
       }
     }
     first_seg = false;
-    }
     if (nwg == 0) return;
-    todo -= u1 - u0;
-    if (todo <= 0) break;
-    u0 = 0;
-    if (++t == ntiles) {
-      t = 0;
-      ++kvh;
-      sidx = 0;
-    }
+    if (!next(u1 - u0)) break;
   }
   if (!by_tile && tid == 0) A.desc[1 + w] = cut_tile;
 }

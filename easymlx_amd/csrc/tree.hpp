@@ -43,7 +43,7 @@ __global__ __launch_bounds__(256) void tree_positions(const int32_t* parents, co
 //
 // One wave per tree, a node to a lane; every step is a comparison and a ballot over the nodes from the last
 // one on, in registers for trees of up to 64 nodes.  Bound by its launch: 3 dependent loads, then some 20
-// cycles per accepted node.
+// cycles per accepted node (one tree of 25: 1.5 us, 32 of up to 60: 3.6).
 template <typename TT>
 __global__ __launch_bounds__(64) void tree_accept(const TT* tokens, const TT* targets, const int32_t* parents,
                                                   const int32_t* qsl, const int n, const int T, int32_t* path,
@@ -150,8 +150,8 @@ struct CommitRowArgs {
 
 // Rows [Hkv, D] of a token-major cache.  Grid (chunks of a row, trees, 2 layers): a thread has one piece of the row
 // and takes its moves in path order, eight loads ahead of their stores: a path ascends, so no store lands on the
-// source of a later move, and no thread touches another's piece.  Bound by latency for one sequence, by the scattered
-// rows' bandwidth for a batch.
+// source of a later move, and no thread touches another's piece.  Bound by latency for one sequence (2 layers: 4.1 us), by
+// the scattered rows' bandwidth for a batch (32 sequences, 32 layers, 61 MB read and written: 8 us, partly from cache).
 template <typename W>
 __global__ __launch_bounds__(128) void tree_commit_rows(CommitRowArgs a) {
   const int l = blockIdx.z >> 1;
