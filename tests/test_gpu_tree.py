@@ -312,3 +312,57 @@ def test_captured_verification(cuda):
             for got, (x, after) in zip(rows_of(v), r):
                 np.testing.assert_array_equal(got, x)
                 np.testing.assert_array_equal(v.kv_lens.cpu().numpy(), after)
+
+
+@pytest.mark.parametrize("kind", ["f16", "q4"])
+def test_captured_decode_with_sinks(cuda, kind):
+    """A decode step with sinks in the metadata, through the compiled proxy and the operator in one graph: every replay
+    gives what the eager views give."""
+    from easymlx_amd import CompiledPagedCacheProxy
+
+    op = OperationRegistry.create("unified_attention")
+    S, hq, hkv, d, page = 5, 8, 2, 64, 16
+    g = torch.Generator().manual_seed(4)
+    make = lambda n: tuple(torch.randn(n, h, d, generator=g).half().to(cuda) for h in (hq, hkv, hkv))  # noqa: E731
+    kw = dict(num_seqs=S, max_seq_len=192, num_kv_heads=hkv, head_dim=d, block_size=page, device=cuda)
+    a, b = (AffinePageCacheView.init(bits=4, group_size=64, **kw) if kind == "q4"
+            else PageCacheView.init(dtype=torch.float16, **kw) for _ in range(2))
+    slots, lens = tuple(range(S)), (60, 1, 100, 33, 7)
+    prompt = make(sum(lens))
+    for v in (a, b):
+        v.concatenate_to_cache(*prompt, cache_metadata=PageMetadata(query_start_loc=None, slot_ids=slots),
+                               slot_ids=slots, query_lens=lens)
+    md = PageMetadata(query_start_loc=torch.arange(S + 1, dtype=torch.int32, device=cuda), slot_ids=slots,
+                      sliding_window=20, sink_tokens=3, is_single_token_decode=True)
+    proxy, buf, out = CompiledPagedCacheProxy(a), make(S), torch.zeros(S, hq, d, dtype=torch.float16, device=cuda)
+
+    def step():
+        q, kc, vc, m = proxy.concatenate_to_cache(*buf, cache_metadata=md)
+        out.copy_(op(query=q, key=kc, value=vc, cache_metadata=m, cache_view=a).attention_outputs)
+
+    def eager():
+        q, kc, vc, m = b.concatenate_to_cache(*buf, cache_metadata=md, slot_ids=slots, query_lens=(1,) * S)
+        return op(query=q, key=kc, value=vc, cache_metadata=m, cache_view=b).attention_outputs
+
+    side = torch.cuda.Stream(cuda)
+    side.wait_stream(torch.cuda.current_stream(cuda))
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    first = eager()
+    assert torch.equal(out, first) and bool(first.abs().sum() > 0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for _ in range(4):
+        for x, y in zip(buf, make(S)):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager()) and torch.equal(a.kv_lens, b.kv_lens)
+        # without its sinks the step gives something else
+        plain = op(query=buf[0], key=b.key_cache, value=b.value_cache, cache_view=b,
+                   cache_metadata=PageMetadata(query_start_loc=md.query_start_loc, block_tables=b.block_tables,
+                                               kv_lens=b.kv_lens, block_size=page, sliding_window=20,
+                                               is_single_token_decode=True)).attention_outputs
+        assert not torch.equal(out, plain)
