@@ -541,17 +541,7 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
   }
 
   int sidx = wide_seq_of(tcum, S, t);
-  auto next = [&](const int done) {  // on to the range's next tile, if there is one
-    todo -= done;
-    u0 = 0;
-    if (++t == ntiles) {
-      t = 0;
-      ++kvh;
-      sidx = 0;
-    }
-    return todo > 0;
-  };
-  for (;;) {
+  while (u0 + todo > kWideBegin) {  // (a range that ends in what it costs to begin a tile leaves it to the next)
     // ---- a segment: blocks [b0, b1) of tile t
     while (tcum[sidx + 1] <= t) ++sidx;
     MaskedSeq sq = wide_seq(A, seqs, __builtin_amdgcn_readfirstlane(sidx));
@@ -564,10 +554,6 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     const MaskedSpan span = masked_span<NT>(mask, past, tok_lo, tok_hi);
     const int nblk = max(1, span.n), u1 = min(nblk + kWideBegin, u0 + min(todo, nblk + kWideBegin - u0));
     const int b0 = max(0, u0 - kWideBegin), b1 = max(0, u1 - kWideBegin);
-    if (b0 == b1) {  // a range that ends in what it costs to begin this tile leaves it to the next
-      if (!next(u1 - u0)) break;
-      continue;
-    }
     const int st_lo = b0, st_hi = min(b1, span.n);  // (an empty tile has a block of nothing)
     const int k_hi = max(past + tok_hi, 0);
     const int32_t* par = mask.parents ? mask.parents + q0 : nullptr;
@@ -1158,7 +1144,13 @@ __global__ __launch_bounds__((WideCfg<C, D, KW, CW>::TH), 2) void masked_wide(Ma
     }
     first_seg = false;
     if (nwg == 0) return;
-    if (!next(u1 - u0)) break;
+    todo -= u1 - u0;
+    u0 = 0;
+    if (++t == ntiles) {
+      t = 0;
+      ++kvh;
+      sidx = 0;
+    }
   }
   if (!by_tile && tid == 0) A.desc[1 + w] = cut_tile;
 }
