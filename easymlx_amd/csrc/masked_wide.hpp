@@ -35,7 +35,7 @@
 //         16, which puts an output off by at most 2^-17 of the largest value it averages: one part would
 //         add an error as large as the output's own rounding).
 // Bound: matrix instructions, 1.5 times the formula's for the second part, at the 1.27 PFLOP/s that a
-// large bf16 product reaches (those 12 trees, 461 GFLOP and 1.04 GB: 543 us of the 740; the matrix units
+// large bf16 product reaches (those 12 trees, 461 GFLOP and 1.04 GB: 543 us of the 746; the matrix units
 // are busy in half of the cycles); over affine pages the vector unit and the chain of a block (codes to
 // values, scores, softmax: 20 vector instructions to a product).
 #pragma once
